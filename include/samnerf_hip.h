@@ -37,6 +37,11 @@ extern "C" {
 #define SNF_ACT_SIGMOID 2
 #define SNF_ACT_GELU 3 /* forward only (nn.GELU, erf form): the image encoder's MLP blocks */
 
+/* element types of the entry points that take more than fp32 */
+#define SNF_F32 0
+#define SNF_BF16 1
+#define SNF_F16 2
+
 typedef void* snf_stream_t;
 
 int snf_version(void);
@@ -508,6 +513,21 @@ int snf_attention_planes(const float* qkv, const float* rel, int Bw, int T, int 
  * inside the kernel, on the matrix cores, from rel_pos_h / rel_pos_w [2n-1][head_dim] (add_decomposed_rel_pos, image_encoder.py:323-361) */
 int snf_attention_planes_rp(const float* qkv, const float* rel_pos_h, const float* rel_pos_w, int Bw, int T, int heads, int head_dim,
                             int n, float scale, uint16_t* out_hi, uint16_t* out_lo, snf_stream_t stream);
+
+/* ---- microscaled 4-bit floats: the encoder's dense layers with both operands in 4 bits (the reference computes them in fp32:
+ *      modeling/image_encoder.py:164-235).
+ * A matrix [M, K] is cut into blocks of 32 along k: 32 e2m1 codes (magnitudes 0 .5 1 1.5 2 3 4 6) and one e8m0 scale byte s for 2^(s-127),
+ *   s = max(floor(log2 max|x|) - 2, -127) + 127,  code = rne(x / 2^(s-127)), magnitudes above 6 become 6;
+ * a block that holds an inf or a NaN has s = 255 and reads back as NaN.  With C = ceil(K / 256):
+ *   codes  uint8 [8 C][M][16]   low nibble first (16-byte aligned);   scales uint8 [C][2][M][4]: byte j of (c, h, row) belongs to block
+ *   8 c + 2 j + h (4-byte aligned).  The columns from K to 256 C hold zeros.
+ * snf_mxfp4_quantize: x [M, K] of `dtype` with rows `ld` elements apart.  snf_mxfp4_dequantize: the values of the codes, out [M, K]
+ *   contiguous.  snf_mxfp4_linear: y [M, N] of `dtype` = act(a w^T + bias), w quantised from [N, K], bias [N] fp32 or NULL, fp32 sums.
+ *   Products below 2^-126 count as zero.  M = 0 is a call without work. */
+int snf_mxfp4_quantize(const void* x, int dtype, int M, int K, int64_t ld, uint8_t* codes, uint8_t* scales, snf_stream_t stream);
+int snf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* out, int dtype, snf_stream_t stream);
+int snf_mxfp4_linear(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* w_codes, const uint8_t* w_scales, const float* bias,
+                     int M, int K, int N, int act, void* y, int dtype, snf_stream_t stream);
 
 /* ---- the batch builder in front of the path (images, feature maps and cameras resident in HBM).
  * snf_pixel_indices: PixelSampler (patch == 1: u [B,3]) / PatchPixelSampler (u [B/patch^2,3]) .sample_method without a

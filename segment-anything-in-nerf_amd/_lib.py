@@ -20,7 +20,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libsamnerf_hip.so")
 HASH_PATH = LIB_PATH + ".srchash"
-SOURCES = ["vit.hip", "gemm_planes.hip", "batch.hip", "sampling.hip", "hashgrid.hip", "fused_head.hip", "linear.hip", "linear_b3.hip", "mlp_chain.hip", "mlp_tiny.hip", "patchconv.hip", "render.hip", "losses.hip", "optim.hip", "streams.hip"]
+SOURCES = ["vit.hip", "mxfp4.hip", "gemm_planes.hip", "batch.hip", "sampling.hip", "hashgrid.hip", "fused_head.hip", "linear.hip", "linear_b3.hip", "mlp_chain.hip", "mlp_tiny.hip", "patchconv.hip", "render.hip", "losses.hip", "optim.hip", "streams.hip"]
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]  # (packed fp32 arithmetic has given wrong results on these cards: scalar only)
 
@@ -156,6 +156,9 @@ SIGNATURES = {
     "snf_layernorm_planes_merge": [P, P, I, I, P, P, F, P, P, P, I, I, I, P],
     "snf_attention_planes": [P, P, I, I, I, I, I, F, P, P, P],
     "snf_attention_planes_rp": [P, P, P, I, I, I, I, I, F, P, P, P],
+    "snf_mxfp4_quantize": [P, I, I, I, c_int64, P, P, P],
+    "snf_mxfp4_dequantize": [P, P, I, I, P, I, P],
+    "snf_mxfp4_linear": [P, P, P, P, P, I, I, I, I, P, I, P],
     "snf_pixel_indices": [P, I, I, I, I, I, P, P],
     "snf_generate_rays": [P, I, P, P, I, P, P, P, P, P],
     "snf_gather_nearest": [P, I, I, I, P, I, I, I, I, I, I, P, P],

@@ -71,6 +71,33 @@ def _chk(t: torch.Tensor, name: str, dtype=torch.float32) -> torch.Tensor:
     return t
 
 
+DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # SNF_F32, SNF_BF16, SNF_F16
+
+
+def _dev(t: torch.Tensor, name: str, device=None) -> torch.device:
+    """The ROCm device of `t`, which has to be the current one (the launches go to its stream) and `device` when given."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: expected a ROCm device tensor; the MI355X path has no CPU fallback")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name}: on {t.device}, the other operands are on {device}")
+    if t.device.index != torch.cuda.current_device():
+        raise RuntimeError(f"{name}: on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return t.device
+
+
+def _stream_on(device: torch.device):
+    """Raw handle of the current stream of `device` (which _dev has found to be the current device)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _rows(t: torch.Tensor):
+    """t [..., C] as (matrix view [R, C] whose rows are contiguous, row stride in elements); copies only what has no such view."""
+    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if m.shape[1] > 1 and m.stride(1) != 1 or m.shape[0] > 1 and m.stride(0) < m.shape[1]:
+        m = m.contiguous()
+    return m, (m.stride(0) if m.shape[0] > 1 else m.shape[1])
+
+
 # --- per-kernel HIP-event timing (bench.py): events are recorded on torch's current stream, which is the stream
 # every kernel is launched on (see _stream()).
 _TIMING = {"names": None, "events": {}}

@@ -1,0 +1,372 @@
+// mxfp4.hip -- microscaled 4-bit floats (gfx950): quantisation, decoding and the product of two quantised matrices.
+//
+// A row is cut into blocks of 32 along k.  A block holds 32 e2m1 codes (sign, magnitude 0 .5 1 1.5 2 3 4 6) and one e8m0 scale byte s
+// that stands for 2^(s - 127):
+//     s = max(floor(log2 max|x|) - 2, -127) + 127,      code = rne(x / 2^(s - 127)), magnitudes above 6 become 6.
+// A block with an infinity or a NaN gets s = 255: all of its values read back as NaN.
+//
+// Layout of a matrix [M, K] (K padded with zeros to Kp = 256 c):
+//     codes  [Kp / 32][M][16]      the 32 codes of (row, block) are 16 consecutive bytes, low nibble first: exactly what a lane hands to
+//                                  v_mfma_scale_f32_32x32x64_f8f6f4 (lane l: row l & 31, block l >> 5), and 64 rows of one block are the
+//                                  1 KB that one global -> LDS copy of a wave moves, in the order in which the fragments are read
+//     scales [Kp / 256][2][M][4]   byte j of (chunk, half, row): block 8 chunk + 2 j + half.  One dword holds a lane's scales of the four
+//                                  k-steps of a 256 chunk; the instruction picks the byte.
+#include "common.hpp"
+
+namespace snf {
+
+typedef float mx_f32x4 __attribute__((ext_vector_type(4)));
+typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
+typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(1))) const void* mx_gptr;
+typedef __attribute__((address_space(3))) void* mx_lptr;
+
+template <typename T>
+struct alignas(16) MxVec {
+    static constexpr int N = 16 / (int)sizeof(T);
+    T v[N];
+};
+
+__device__ __forceinline__ int mx_scale_byte(uint32_t amax_bits) {
+    const int e = (int)(amax_bits >> 23);  // biased exponent of the block's largest magnitude (0: zero or subnormal)
+    return e == 255 ? 255 : max(e - 2, 0);
+}
+// 2^(byte - 127) as a float (byte < 255; byte 0 is the subnormal 2^-127)
+__device__ __forceinline__ float mx_scale_float(int byte) { return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u); }
+
+// ---- quantisation ---------------------------------------------------------------------------------------------------------------
+// A workgroup takes 32 rows x 256 columns.  A lane loads 16 bytes of a row (whole rows of the tile are contiguous), the lanes of a block
+// agree on its largest magnitude by cross-lane exchanges, convert their own values and put the codes into LDS in the order of the layout;
+// the tile leaves as 8 runs of 32 x 16 bytes.
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(256) void k_mxfp4_quantize(const T* __restrict__ x, int M, int K, int64_t ld, int chunks,
+                                                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    constexpr int V = MxVec<T>::N, LPR = 256 / V, RPP = 256 / LPR, LPB = 32 / V;
+    constexpr int KB_PITCH = 32 * 16 + 16;  // (one 16-byte column further per block: the eight blocks of a row lie in different banks)
+    __shared__ __attribute__((aligned(16))) uint8_t s_codes[8 * KB_PITCH];
+    __shared__ __attribute__((aligned(16))) uint8_t s_scales[2 * 32 * 4];
+    const int c = (int)(blockIdx.x % (unsigned)chunks);
+    const int r0 = (int)(blockIdx.x / (unsigned)chunks) * 32;
+    const int lr = threadIdx.x / LPR, lc = threadIdx.x % LPR;
+    const int col = c * 256 + lc * V, kb = lc / LPB, part = lc % LPB;
+    float v[32 / RPP][V];
+#pragma unroll
+    for (int p = 0; p < 32 / RPP; ++p) {
+        const int row = r0 + p * RPP + lr;
+        const bool live = row < M;
+        const T* src = x + (int64_t)row * ld + col;
+        if (WIDE && live && col + V <= K) {
+            const MxVec<T> t = *reinterpret_cast<const MxVec<T>*>(src);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[p][i] = (float)t.v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[p][i] = live && col + i < K ? (float)src[i] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < 32 / RPP; ++p) {
+        uint32_t amax = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) amax = max(amax, __float_as_uint(v[p][i]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int d = 1; d < LPB; d <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, d, WAVE));
+        const int sb = mx_scale_byte(amax);
+        const float sc = mx_scale_float(sb);
+        uint32_t w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[p][0], v[p][1], sc, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[p][2], v[p][3], sc, 1);
+        if constexpr (V == 8) {
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[p][4], v[p][5], sc, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[p][6], v[p][7], sc, 3);
+        }
+        if (sb == 255) w = 0x77777777u;  // (any non-zero magnitude: NaN under a NaN scale)
+        const int lrow = p * RPP + lr;
+        uint8_t* dst = s_codes + kb * KB_PITCH + lrow * 16 + part * (V / 2);
+        if constexpr (V == 8) *reinterpret_cast<uint32_t*>(dst) = w;
+        else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w;
+        if (part == 0) s_scales[((kb & 1) * 32 + lrow) * 4 + (kb >> 1)] = (uint8_t)sb;
+    }
+    __syncthreads();
+    {
+        const int b = threadIdx.x >> 5, r = threadIdx.x & 31;
+        if (r0 + r < M)
+            *reinterpret_cast<uint4*>(codes + (((size_t)c * 8 + b) * M + r0 + r) * 16) =
+                *reinterpret_cast<const uint4*>(s_codes + b * KB_PITCH + r * 16);
+    }
+    if (threadIdx.x < 64) {
+        const int h = threadIdx.x >> 5, r = threadIdx.x & 31;
+        if (r0 + r < M)
+            reinterpret_cast<uint32_t*>(scales)[((size_t)c * 2 + h) * M + r0 + r] = reinterpret_cast<const uint32_t*>(s_scales)[h * 32 + r];
+    }
+}
+
+// ---- decoding -------------------------------------------------------------------------------------------------------------------
+// The tiles of the quantisation, the other way: codes and scales of 32 rows x 256 columns into LDS, rows out.
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(256) void k_mxfp4_dequantize(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int M,
+                                                          int K, int chunks, T* __restrict__ out) {
+    constexpr int V = MxVec<T>::N, LPR = 256 / V, RPP = 256 / LPR, LPB = 32 / V;
+    constexpr int KB_PITCH = 32 * 16 + 16;
+    __shared__ __attribute__((aligned(16))) uint8_t s_codes[8 * KB_PITCH];
+    __shared__ __attribute__((aligned(16))) uint8_t s_scales[2 * 32 * 4];
+    const int c = (int)(blockIdx.x % (unsigned)chunks);
+    const int r0 = (int)(blockIdx.x / (unsigned)chunks) * 32;
+    {
+        const int b = threadIdx.x >> 5, r = threadIdx.x & 31;
+        if (r0 + r < M)
+            *reinterpret_cast<uint4*>(s_codes + b * KB_PITCH + r * 16) =
+                *reinterpret_cast<const uint4*>(codes + (((size_t)c * 8 + b) * M + r0 + r) * 16);
+    }
+    if (threadIdx.x < 64) {
+        const int h = threadIdx.x >> 5, r = threadIdx.x & 31;
+        if (r0 + r < M)
+            reinterpret_cast<uint32_t*>(s_scales)[h * 32 + r] = reinterpret_cast<const uint32_t*>(scales)[((size_t)c * 2 + h) * M + r0 + r];
+    }
+    __syncthreads();
+    const int lr = threadIdx.x / LPR, lc = threadIdx.x % LPR;
+    const int col = c * 256 + lc * V, kb = lc / LPB, part = lc % LPB;
+#pragma unroll
+    for (int p = 0; p < 32 / RPP; ++p) {
+        const int lrow = p * RPP + lr, row = r0 + lrow;
+        if (row >= M || col >= K) continue;
+        const uint8_t* src = s_codes + kb * KB_PITCH + lrow * 16 + part * (V / 2);
+        const uint32_t w = V == 8 ? *reinterpret_cast<const uint32_t*>(src) : (uint32_t)*reinterpret_cast<const uint16_t*>(src);
+        const int sb = s_scales[((kb & 1) * 32 + lrow) * 4 + (kb >> 1)];
+        const float sc = sb == 255 ? __uint_as_float(0x7FC00000u) : mx_scale_float(sb);
+        MxVec<T> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            // magnitudes: codes 0, 1 are 0 and 1/2, the others (1 + m / 2) 2^(e - 1)
+            const uint32_t q = (w >> (4 * i)) & 15u, e = (q >> 1) & 3u, m = q & 1u;
+            const float mag = e == 0 ? 0.5f * (float)m : __uint_as_float(((e + 126u) << 23) | (m << 22));
+            o.v[i] = (T)((q & 8u ? -mag : mag) * sc);
+        }
+        T* dst = out + (int64_t)row * K + col;
+        if (WIDE && col + V <= K) {
+            *reinterpret_cast<MxVec<T>*>(dst) = o;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (col + i < K) dst[i] = o.v[i];
+        }
+    }
+}
+
+// ---- product --------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float mx_act(float v, int act) {
+    switch (act) {
+        case SNF_ACT_RELU: return v > 0.f || v != v ? v : 0.f;
+        case SNF_ACT_SIGMOID: return 1.f / (1.f + expf(-v));
+        case SNF_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+        default: return v;
+    }
+}
+
+// y[m][n] = act(sum_k a[m][k] w[n][k] + bias[n]), fp32 sums on v_mfma_scale_f32_32x32x64_f8f6f4 (products of codes are exact).
+// A workgroup of four waves (2 x 2) takes BM rows x BN columns, a wave (BM / 2) x (BN / 2); a stage is 256 k of both operands in LDS, two
+// stage buffers: the copies of the next stage run under the products of this one.  The weights are the instruction's first operand, so a
+// lane ends up with four consecutive columns of one row.
+template <int BM, int BN, typename T>
+__global__ __launch_bounds__(256) void k_mxfp4_linear(const uint8_t* __restrict__ a, const uint8_t* __restrict__ as,
+                                                      const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
+                                                      const float* __restrict__ bias, int M, int N, int chunks, int act,
+                                                      T* __restrict__ y, int row_tiles, int col_tiles) {
+    constexpr int RB = BM / 64, CB = BN / 64;  // 32-row / 32-column blocks of a wave
+    constexpr int A_BYTES = 8 * BM * 16, W_BYTES = 8 * BN * 16, STAGE = A_BYTES + W_BYTES;
+    extern __shared__ __attribute__((aligned(16))) uint8_t mx_lds[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 31, half = lane >> 5, wr = wave >> 1, wc = wave & 1;
+    // consecutive tiles of one XCD share their rows' operand in its L2
+    const int total = row_tiles * col_tiles, per = (total + 7) >> 3;
+    const int slot = (int)blockIdx.x >> 3, t = ((int)blockIdx.x & 7) * per + slot;
+    if (slot >= per || t >= total) return;
+    const int rt = t / col_tiles, ct = t - rt * col_tiles;
+    const int m0 = rt * BM, n0 = ct * BN;
+
+    mx_f32x16 acc[RB][CB];
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    // rows past the end read the last row (their results are not stored)
+    auto copy = [&](int c, int buf) {
+        uint8_t* dst = mx_lds + buf * STAGE;
+#pragma unroll
+        for (int p = 0; p < 8 * (BM / 64) / 4; ++p) {
+            const int piece = p * 4 + wave, kb = piece / (BM / 64), g = piece % (BM / 64);
+            const int row = min(m0 + g * 64 + lane, M - 1);
+            __builtin_amdgcn_global_load_lds((mx_gptr)(a + (((size_t)c * 8 + kb) * M + row) * 16), (mx_lptr)(dst + (kb * BM + g * 64) * 16), 16,
+                                             0, 0);
+        }
+#pragma unroll
+        for (int p = 0; p < 8 * (BN / 64) / 4; ++p) {
+            const int piece = p * 4 + wave, kb = piece / (BN / 64), g = piece % (BN / 64);
+            const int row = min(n0 + g * 64 + lane, N - 1);
+            __builtin_amdgcn_global_load_lds((mx_gptr)(w + (((size_t)c * 8 + kb) * N + row) * 16),
+                                             (mx_lptr)(dst + A_BYTES + (kb * BN + g * 64) * 16), 16, 0, 0);
+        }
+    };
+    int arow[RB], wrow[CB];
+#pragma unroll
+    for (int i = 0; i < RB; ++i) arow[i] = min(m0 + wr * (BM / 2) + i * 32 + li, M - 1);
+#pragma unroll
+    for (int j = 0; j < CB; ++j) wrow[j] = min(n0 + wc * (BN / 2) + j * 32 + li, N - 1);
+    const int* as32 = reinterpret_cast<const int*>(as);
+    const int* ws32 = reinterpret_cast<const int*>(ws);
+
+    copy(0, 0);
+    __syncthreads();
+    for (int c = 0; c < chunks; ++c) {
+        if (c + 1 < chunks) copy(c + 1, (c + 1) & 1);
+        int sa[RB], sw[CB];
+#pragma unroll
+        for (int i = 0; i < RB; ++i) sa[i] = as32[((size_t)c * 2 + half) * M + arow[i]];
+#pragma unroll
+        for (int j = 0; j < CB; ++j) sw[j] = ws32[((size_t)c * 2 + half) * N + wrow[j]];
+        const uint8_t* fa = mx_lds + (c & 1) * STAGE + (half * BM + wr * (BM / 2) + li) * 16;
+        const uint8_t* fw = mx_lds + (c & 1) * STAGE + A_BYTES + (half * BN + wc * (BN / 2) + li) * 16;
+        // the scale's byte is part of the instruction
+#define MX_STEP(S_)                                                                                                              \
+    {                                                                                                                            \
+        mx_i32x8 xa[RB], xw[CB];                                                                                                 \
+        _Pragma("unroll") for (int i = 0; i < RB; ++i) {                                                                         \
+            const int4 q = *reinterpret_cast<const int4*>(fa + ((S_) * 2 * BM + i * 32) * 16);                                   \
+            xa[i] = mx_i32x8{q.x, q.y, q.z, q.w, 0, 0, 0, 0};                                                                    \
+        }                                                                                                                        \
+        _Pragma("unroll") for (int j = 0; j < CB; ++j) {                                                                         \
+            const int4 q = *reinterpret_cast<const int4*>(fw + ((S_) * 2 * BN + j * 32) * 16);                                   \
+            xw[j] = mx_i32x8{q.x, q.y, q.z, q.w, 0, 0, 0, 0};                                                                    \
+        }                                                                                                                        \
+        _Pragma("unroll") for (int i = 0; i < RB; ++i) _Pragma("unroll") for (int j = 0; j < CB; ++j) acc[i][j] =                \
+            __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xw[j], xa[i], acc[i][j], 4, 4, S_, sw[j], S_, sa[i]);                \
+    }
+        MX_STEP(0)
+        MX_STEP(1)
+        MX_STEP(2)
+        MX_STEP(3)
+#undef MX_STEP
+        __syncthreads();
+    }
+    // element e of a lane: column 8 (e / 4) + 4 half + e % 4 of the block, row li
+    const bool wide = N % 4 == 0;
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+        const int m = m0 + wr * (BM / 2) + i * 32 + li;
+        if (m >= M) continue;
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int n = n0 + wc * (BN / 2) + j * 32 + 8 * g + 4 * half;
+                struct alignas(4 * sizeof(T)) { T v[4]; } o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o.v[e] = (T)mx_act(acc[i][j][4 * g + e] + (bias && n + e < N ? bias[n + e] : 0.f), act);
+                T* dst = y + (int64_t)m * N + n;
+                if (wide) {
+                    if (n < N) *reinterpret_cast<decltype(o)*>(dst) = o;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n + e < N) dst[e] = o.v[e];
+                }
+            }
+    }
+}
+
+static bool mx_aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+template <typename T>
+static int mx_quantize_t(const T* x, int M, int K, int64_t ld, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+    const int chunks = ceil_div(K, 256);
+    const int64_t blocks = (int64_t)ceil_div(M, 32) * chunks;
+    SNF_REQUIRE(blocks < ((int64_t)1 << 31), "snf_mxfp4_quantize: %d x %d is too large for one launch", M, K);
+    if (mx_aligned(x, 16) && (ld * (int64_t)sizeof(T)) % 16 == 0)
+        k_mxfp4_quantize<T, true><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(x, M, K, ld, chunks, codes, scales);
+    else
+        k_mxfp4_quantize<T, false><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(x, M, K, ld, chunks, codes, scales);
+    SNF_LAUNCH_CHECK("snf_mxfp4_quantize");
+    return SNF_OK;
+}
+
+template <typename T>
+static int mx_dequantize_t(const uint8_t* codes, const uint8_t* scales, int M, int K, T* out, hipStream_t st) {
+    const int chunks = ceil_div(K, 256);
+    const int64_t blocks = (int64_t)ceil_div(M, 32) * chunks;
+    SNF_REQUIRE(blocks < ((int64_t)1 << 31), "snf_mxfp4_dequantize: %d x %d is too large for one launch", M, K);
+    if (mx_aligned(out, 16) && ((int64_t)K * (int64_t)sizeof(T)) % 16 == 0)
+        k_mxfp4_dequantize<T, true><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(codes, scales, M, K, chunks, out);
+    else
+        k_mxfp4_dequantize<T, false><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(codes, scales, M, K, chunks, out);
+    SNF_LAUNCH_CHECK("snf_mxfp4_dequantize");
+    return SNF_OK;
+}
+
+template <typename T>
+static int mx_linear_t(const uint8_t* a, const uint8_t* as, const uint8_t* w, const uint8_t* ws, const float* bias, int M, int K, int N,
+                       int act, T* y, hipStream_t st) {
+    constexpr int BM = 128, BN = 128;
+    const int chunks = ceil_div(K, 256), rts = ceil_div(M, BM), cts = ceil_div(N, BN);
+    SNF_REQUIRE((int64_t)rts * cts < ((int64_t)1 << 30), "snf_mxfp4_linear: %d x %d is too large for one launch", M, N);
+    const int per = (rts * cts + 7) / 8;
+    k_mxfp4_linear<BM, BN, T><<<dim3(8 * per), dim3(256), 2 * 8 * (BM + BN) * 16, st>>>(a, as, w, ws, bias, M, N, chunks, act, y, rts, cts);
+    SNF_LAUNCH_CHECK("snf_mxfp4_linear");
+    return SNF_OK;
+}
+
+}  // namespace snf
+
+extern "C" {
+
+int snf_mxfp4_quantize(const void* x, int dtype, int M, int K, int64_t ld, uint8_t* codes, uint8_t* scales, snf_stream_t stream) {
+    SNF_REQUIRE(M >= 0 && K >= 1, "snf_mxfp4_quantize: bad sizes M=%d K=%d", M, K);
+    if (M == 0) return SNF_OK;
+    SNF_REQUIRE(x && codes && scales, "snf_mxfp4_quantize: null pointer");
+    SNF_REQUIRE(ld >= K || M == 1, "snf_mxfp4_quantize: rows of %d values overlap at stride %lld", K, (long long)ld);
+    SNF_REQUIRE(snf::mx_aligned(codes, 16) && snf::mx_aligned(scales, 4), "snf_mxfp4_quantize: codes / scales are not aligned");
+    hipStream_t st = (hipStream_t)stream;
+    switch (dtype) {
+        case SNF_F32: return snf::mx_quantize_t((const float*)x, M, K, ld, codes, scales, st);
+        case SNF_BF16: return snf::mx_quantize_t((const __bf16*)x, M, K, ld, codes, scales, st);
+        case SNF_F16: return snf::mx_quantize_t((const _Float16*)x, M, K, ld, codes, scales, st);
+    }
+    SNF_REQUIRE(false, "snf_mxfp4_quantize: unknown dtype %d", dtype);
+}
+
+int snf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* out, int dtype, snf_stream_t stream) {
+    SNF_REQUIRE(M >= 0 && K >= 1, "snf_mxfp4_dequantize: bad sizes M=%d K=%d", M, K);
+    if (M == 0) return SNF_OK;
+    SNF_REQUIRE(out && codes && scales, "snf_mxfp4_dequantize: null pointer");
+    SNF_REQUIRE(snf::mx_aligned(codes, 16) && snf::mx_aligned(scales, 4), "snf_mxfp4_dequantize: codes / scales are not aligned");
+    hipStream_t st = (hipStream_t)stream;
+    switch (dtype) {
+        case SNF_F32: return snf::mx_dequantize_t(codes, scales, M, K, (float*)out, st);
+        case SNF_BF16: return snf::mx_dequantize_t(codes, scales, M, K, (__bf16*)out, st);
+        case SNF_F16: return snf::mx_dequantize_t(codes, scales, M, K, (_Float16*)out, st);
+    }
+    SNF_REQUIRE(false, "snf_mxfp4_dequantize: unknown dtype %d", dtype);
+}
+
+int snf_mxfp4_linear(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* w_codes, const uint8_t* w_scales, const float* bias,
+                     int M, int K, int N, int act, void* y, int dtype, snf_stream_t stream) {
+    SNF_REQUIRE(M >= 0 && K >= 1 && N >= 1, "snf_mxfp4_linear: bad sizes M=%d K=%d N=%d", M, K, N);
+    SNF_REQUIRE(act >= SNF_ACT_NONE && act <= SNF_ACT_GELU, "snf_mxfp4_linear: unknown activation %d", act);
+    if (M == 0) return SNF_OK;
+    SNF_REQUIRE(a_codes && a_scales && w_codes && w_scales && y, "snf_mxfp4_linear: null pointer");
+    SNF_REQUIRE(snf::mx_aligned(a_codes, 16) && snf::mx_aligned(w_codes, 16) && snf::mx_aligned(a_scales, 4) && snf::mx_aligned(w_scales, 4) &&
+                    snf::mx_aligned(y, 16),
+                "snf_mxfp4_linear: an operand is not aligned");
+    hipStream_t st = (hipStream_t)stream;
+    switch (dtype) {
+        case SNF_F32: return snf::mx_linear_t(a_codes, a_scales, w_codes, w_scales, bias, M, K, N, act, (float*)y, st);
+        case SNF_BF16: return snf::mx_linear_t(a_codes, a_scales, w_codes, w_scales, bias, M, K, N, act, (__bf16*)y, st);
+        case SNF_F16: return snf::mx_linear_t(a_codes, a_scales, w_codes, w_scales, bias, M, K, N, act, (_Float16*)y, st);
+    }
+    SNF_REQUIRE(false, "snf_mxfp4_linear: unknown dtype %d", dtype);
+}
+
+}  // extern "C"

@@ -30,6 +30,7 @@ from .ops_data import *  # noqa: F401,F403
 from .ops_losses import *  # noqa: F401,F403
 from .ops_losses import _Distortion, _Interlevel, _RowMSELoss  # noqa: F401
 from .ops_optim import *  # noqa: F401,F403
+from .ops_quant import *  # noqa: F401,F403
 from .ops_render import *  # noqa: F401,F403
 from .ops_render import _CompositeRGB, _FeatureMean, _HeadInput, _TruncExpSel, _Weights  # noqa: F401
 from .ops_sampling import *  # noqa: F401,F403

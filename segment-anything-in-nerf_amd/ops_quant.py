@@ -1,0 +1,124 @@
+"""Microscaled 4-bit floats (csrc/mxfp4.hip): quantisation, decoding and dense layers with both operands in that format -- inference
+only, like the encoder pieces of ops_vit (`samnerf_amd.ops` re-exports everything here)."""
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+
+from ._opcore import ACT_GELU, ACT_NONE, DTYPE_CODE, _dev, _launch, _p, _rows, _stream_on
+
+__all__ = ["MXFP4_BLOCK", "Mxfp4", "quantize_mxfp4", "dequantize_mxfp4", "linear_mxfp4"]
+
+MXFP4_BLOCK = 32  # values that share a scale
+
+
+class Mxfp4:
+    """A matrix [M, K] in blocks of 32 values along K: e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign), one power-of-two scale a block.
+
+    codes uint8 [8 C, M, 16] and scales uint8 [2 C, M, 4], C = ceil(K / 256), in the order in which the product reads them (the layout
+    stands in include/samnerf_hip.h); `shape` is the shape of the tensor that was quantised.  17 / 32 byte a value."""
+    __slots__ = ("codes", "scales", "M", "K", "shape")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, K: int, shape: Optional[Tuple[int, ...]] = None):
+        chunks = -(-int(K) // 256)
+        if K < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("Mxfp4: K >= 1, uint8 codes and uint8 scales expected")
+        if codes.dim() != 3 or codes.shape[0] != 8 * chunks or codes.shape[2] != 16:
+            raise ValueError(f"Mxfp4: codes of K={K} have shape [{8 * chunks}, M, 16], got {tuple(codes.shape)}")
+        self.M, self.K = int(codes.shape[1]), int(K)
+        if tuple(scales.shape) != (2 * chunks, self.M, 4):
+            raise ValueError(f"Mxfp4: scales of [{self.M}, {K}] have shape [{2 * chunks}, {self.M}, 4], got {tuple(scales.shape)}")
+        if codes.device != scales.device or not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError("Mxfp4: codes and scales are contiguous and on one device")
+        self.shape = tuple(shape) if shape is not None else (self.M, self.K)
+        n = 1
+        for d in self.shape[:-1]:
+            n *= d
+        if self.shape[-1] != self.K or n != self.M:
+            raise ValueError(f"Mxfp4: {self.shape} is not a shape of {self.M} rows of {self.K}")
+        self.codes, self.scales = codes, scales
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def float(self) -> torch.Tensor:
+        """The values as float32, in the shape that was quantised."""
+        return dequantize_mxfp4(self)
+
+
+@torch.no_grad()
+def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
+    """x [..., K] (float32 / bfloat16 / float16; rows may be strided) -> Mxfp4.  Per block of 32 along K the scale is
+    2^max(floor(log2 max|x|) - 2, -127); values are rounded to the nearest code (halves to even), magnitudes above 6 scales become 6.
+    Blocks with an infinity or a NaN become NaN as a whole.  The last block of a K that 32 does not divide is filled with zeros."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in DTYPE_CODE:
+        raise TypeError(f"quantize_mxfp4: float32, bfloat16 or float16 expected, got {getattr(x, 'dtype', type(x))}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"quantize_mxfp4: rows of at least one value expected, got {tuple(x.shape)}")
+    dev = _dev(x, "x")
+    shape, K = tuple(x.shape), int(x.shape[-1])
+    if x.dim() == 1:
+        x = x.unsqueeze(0)
+    M = x.numel() // K
+    chunks = -(-K // 256)
+    codes = torch.empty((8 * chunks, M, 16), device=dev, dtype=torch.uint8)
+    scales = torch.empty((2 * chunks, M, 4), device=dev, dtype=torch.uint8)
+    if M:
+        x, ld = _rows(x)
+        _launch("snf_mxfp4_quantize", _p(x), DTYPE_CODE[x.dtype], M, K, ld, _p(codes), _p(scales), _stream_on(dev),
+                units=float(M * K * x.element_size()))
+    return Mxfp4(codes, scales, K, shape)
+
+
+@torch.no_grad()
+def dequantize_mxfp4(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values that `q` holds, in its shape.  float32 holds every value exactly; so does the type that was quantised."""
+    if not isinstance(q, Mxfp4):
+        raise TypeError(f"dequantize_mxfp4: an Mxfp4 expected, got {type(q)}")
+    if dtype not in DTYPE_CODE:
+        raise TypeError(f"dequantize_mxfp4: float32, bfloat16 or float16 expected, got {dtype}")
+    dev = _dev(q.codes, "q")
+    out = torch.empty(q.shape, device=dev, dtype=dtype)
+    if q.M:
+        _launch("snf_mxfp4_dequantize", _p(q.codes), _p(q.scales), q.M, q.K, _p(out), DTYPE_CODE[dtype], _stream_on(dev),
+                units=float(out.numel() * out.element_size()))
+    return out
+
+
+@torch.no_grad()
+def linear_mxfp4(x: Union[torch.Tensor, Mxfp4], w: Mxfp4, bias: Optional[torch.Tensor] = None, act: int = ACT_NONE,
+                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(x W^T + bias) with both operands in 4 bits and float32 sums: x [..., K] is quantised on the way in (or comes as an Mxfp4),
+    w = quantize_mxfp4(weight [N, K]) once per checkpoint, bias [N] float32, act one of ops.ACT_*.  The result [..., N] has x's type
+    (float32 for an Mxfp4) unless out_dtype says otherwise."""
+    if not isinstance(w, Mxfp4) or len(w.shape) != 2:
+        raise TypeError("linear_mxfp4: w is quantize_mxfp4(weight) of a weight [N, K]")
+    if not isinstance(x, Mxfp4):
+        if not isinstance(x, torch.Tensor) or x.dtype not in DTYPE_CODE:
+            raise TypeError(f"linear_mxfp4: x is float32, bfloat16, float16 or an Mxfp4, got {getattr(x, 'dtype', type(x))}")
+    if len(x.shape) < 1 or x.shape[-1] != w.K:
+        raise ValueError(f"linear_mxfp4: x {tuple(x.shape)} does not end in the weight's {w.K} columns")
+    if w.M < 1:
+        raise ValueError("linear_mxfp4: a weight without rows")
+    if not ACT_NONE <= int(act) <= ACT_GELU:
+        raise ValueError(f"linear_mxfp4: unknown activation {act}")
+    if out_dtype is None:
+        out_dtype = torch.float32 if isinstance(x, Mxfp4) else x.dtype
+    if out_dtype not in DTYPE_CODE:
+        raise TypeError(f"linear_mxfp4: the result is float32, bfloat16 or float16, not {out_dtype}")
+    dev = _dev(w.codes, "w")
+    _dev(x.codes if isinstance(x, Mxfp4) else x, "x", dev)
+    if bias is not None:
+        _dev(bias, "bias", dev)
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (w.M,):
+            raise ValueError(f"linear_mxfp4: bias is float32 [{w.M}], got {bias.dtype} {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    y = torch.empty(tuple(x.shape[:-1]) + (w.M,), device=dev, dtype=out_dtype)
+    if y.numel() == 0:
+        return y
+    q = x if isinstance(x, Mxfp4) else quantize_mxfp4(x)
+    _launch("snf_mxfp4_linear", _p(q.codes), _p(q.scales), _p(w.codes), _p(w.scales), _p(bias), q.M, q.K, w.M, int(act), _p(y),
+            DTYPE_CODE[out_dtype], _stream_on(dev), tag=f"{q.K}x{w.M}", units=2.0 * q.M * q.K * w.M)
+    return y
