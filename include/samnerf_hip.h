@@ -514,6 +514,36 @@ int snf_attention_planes(const float* qkv, const float* rel, int Bw, int T, int 
 int snf_attention_planes_rp(const float* qkv, const float* rel_pos_h, const float* rel_pos_w, int Bw, int T, int heads, int head_dim,
                             int n, float scale, uint16_t* out_hi, uint16_t* out_lo, snf_stream_t stream);
 
+/* ---- a teacher's top logits, and distillation from them (beside the L2 distillation losses, snf_rowmse_loss_*): the targets of a row are
+ *      the k largest of the teacher's V logits and the mass of all the others.
+ * snf_top_logits: x [R, V] of `dtype`, rows `ld` elements apart -> ids [R, k] int32 and logits [R, k] of `dtype`, largest first (equal
+ *   logits: the lowest place first; a NaN is above everything), rest [R] = log sum exp(x / temperature) over all other places (-inf: none).
+ *   workspace: snf_top_logits_workspace_bytes(...) bytes, 8-byte aligned.  1 <= k <= min(V, 256), V <= SNF_TOP_MAX_V.
+ * snf_top_distill_fwd: z [R, V] of `dtype` a student's logits; ids [R, K] (int64 where ids_wide, else int32; negative: no entry), top
+ *   [R, K] of top_dtype, rest [R] or NULL.  With p = softmax over the row's entries of (top / T [, rest]), q = softmax(z / T), q_rest =
+ *   sum of q over the places that the row's ids do not name:
+ *     rows[r] = weight T^2 ( sum_k p_k (log p_k - log q_ids_k) + p_rest (log p_rest - log q_rest) )
+ *   without rest, p sums to 1 over the entries.  Rows without an entry, or whose teacher has no mass, are no targets: rows = counted = 0.
+ *   An id >= V makes its row NaN.  stats [R, 4] (16-byte aligned) and p [R, K] are kept for the backward pass.  workspace:
+ *   snf_top_distill_workspace_bytes(...) bytes, 8-byte aligned.
+ * snf_top_distill_mean: loss[0] = sum of rows / divisor[0], divisor[0] = number of counted rows (at least 1) or, mean == 0, 1.
+ * snf_top_distill_bwd: dz [R, V] contiguous of `dtype` = g weight T (q_v - sum_{k: ids_k = v} p_k - (v not named) p_rest q_v / q_rest),
+ *   divided by divisor[0] where divisor (of snf_top_distill_mean) is given; g [1], or [R] where g_per_row.  Rows that are no
+ *   targets get zeros. */
+#define SNF_TOP_MAX_V 1000000
+int64_t snf_top_logits_workspace_bytes(int R, int V, int k, int dtype);
+int snf_top_logits(const void* x, int dtype, int R, int V, int64_t ld, int k, float temperature, int32_t* ids, void* logits, float* rest,
+                   void* workspace, int64_t workspace_bytes, snf_stream_t stream);
+int64_t snf_top_distill_workspace_bytes(int R, int V, int dtype);
+int snf_top_distill_fwd(const void* z, int dtype, int R, int V, int64_t ld, const void* ids, int ids_wide, const void* top, int top_dtype,
+                        const float* rest, int K, float temperature, float weight, float* rows, float* counted, float* stats, float* p,
+                        void* workspace, int64_t workspace_bytes, snf_stream_t stream);
+int snf_top_distill_mean(const float* rows, const float* counted, int R, int mean, float* loss, float* divisor,
+                         snf_stream_t stream);
+int snf_top_distill_bwd(const void* z, int dtype, int R, int V, int64_t ld, const void* ids, int ids_wide, int K, float temperature,
+                        float weight, const float* g, int g_per_row, const float* divisor, const float* counted, const float* stats,
+                        const float* p, void* dz, snf_stream_t stream);
+
 /* ---- microscaled 4-bit floats: the encoder's dense layers with both operands in 4 bits (the reference computes them in fp32:
  *      modeling/image_encoder.py:164-235).
  * A matrix [M, K] is cut into blocks of 32 along k: 32 e2m1 codes (magnitudes 0 .5 1 1.5 2 3 4 6) and one e8m0 scale byte s for 2^(s-127),

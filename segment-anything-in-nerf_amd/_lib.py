@@ -20,7 +20,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libsamnerf_hip.so")
 HASH_PATH = LIB_PATH + ".srchash"
-SOURCES = ["vit.hip", "mxfp4.hip", "gemm_planes.hip", "batch.hip", "sampling.hip", "hashgrid.hip", "fused_head.hip", "linear.hip", "linear_b3.hip", "mlp_chain.hip", "mlp_tiny.hip", "patchconv.hip", "render.hip", "losses.hip", "optim.hip", "streams.hip"]
+SOURCES = ["vit.hip", "mxfp4.hip", "gemm_planes.hip", "batch.hip", "sampling.hip", "hashgrid.hip", "fused_head.hip", "linear.hip", "linear_b3.hip", "mlp_chain.hip", "mlp_tiny.hip", "patchconv.hip", "render.hip", "losses.hip", "distill.hip", "optim.hip", "streams.hip"]
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]  # (packed fp32 arithmetic has given wrong results on these cards: scalar only)
 
@@ -156,6 +156,10 @@ SIGNATURES = {
     "snf_layernorm_planes_merge": [P, P, I, I, P, P, F, P, P, P, I, I, I, P],
     "snf_attention_planes": [P, P, I, I, I, I, I, F, P, P, P],
     "snf_attention_planes_rp": [P, P, P, I, I, I, I, I, F, P, P, P],
+    "snf_top_logits": [P, I, I, I, c_int64, I, F, P, P, P, P, c_int64, P],
+    "snf_top_distill_fwd": [P, I, I, I, c_int64, P, I, P, I, P, I, F, F, P, P, P, P, P, c_int64, P],
+    "snf_top_distill_mean": [P, P, I, I, P, P, P],
+    "snf_top_distill_bwd": [P, I, I, I, c_int64, P, I, I, F, F, P, I, P, P, P, P, P, P],
     "snf_mxfp4_quantize": [P, I, I, I, c_int64, P, P, P],
     "snf_mxfp4_dequantize": [P, P, I, I, P, I, P],
     "snf_mxfp4_linear": [P, P, P, P, P, I, I, I, I, P, I, P],
@@ -209,6 +213,10 @@ def load(auto_build: bool = True) -> ctypes.CDLL:
     lib.snf_mlp64_bwd_fused_workspace_bytes.argtypes = [c_int]
     lib.snf_linear_bwd_weight_workspace_bytes.restype = c_int64
     lib.snf_linear_bwd_weight_workspace_bytes.argtypes = [c_int, c_int, c_int]
+    lib.snf_top_logits_workspace_bytes.restype = c_int64
+    lib.snf_top_logits_workspace_bytes.argtypes = [c_int, c_int, c_int, c_int]
+    lib.snf_top_distill_workspace_bytes.restype = c_int64
+    lib.snf_top_distill_workspace_bytes.argtypes = [c_int, c_int, c_int]
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)  # AttributeError if a declared symbol is not exported
         fn.restype = c_int

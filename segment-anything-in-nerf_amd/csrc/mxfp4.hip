@@ -284,7 +284,7 @@ template <typename T>
 static int mx_quantize_t(const T* x, int M, int K, int64_t ld, uint8_t* codes, uint8_t* scales, hipStream_t st) {
     const int chunks = ceil_div(K, 256);
     const int64_t blocks = (int64_t)ceil_div(M, 32) * chunks;
-    SNF_REQUIRE(blocks < ((int64_t)1 << 31), "snf_mxfp4_quantize: %d x %d is too large for one launch", M, K);
+    SNF_REQUIRE(blocks * 256 < ((int64_t)1 << 32), "snf_mxfp4_quantize: %d x %d is too large for one launch", M, K);
     if (mx_aligned(x, 16) && (ld * (int64_t)sizeof(T)) % 16 == 0)
         k_mxfp4_quantize<T, true><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(x, M, K, ld, chunks, codes, scales);
     else
@@ -297,7 +297,7 @@ template <typename T>
 static int mx_dequantize_t(const uint8_t* codes, const uint8_t* scales, int M, int K, T* out, hipStream_t st) {
     const int chunks = ceil_div(K, 256);
     const int64_t blocks = (int64_t)ceil_div(M, 32) * chunks;
-    SNF_REQUIRE(blocks < ((int64_t)1 << 31), "snf_mxfp4_dequantize: %d x %d is too large for one launch", M, K);
+    SNF_REQUIRE(blocks * 256 < ((int64_t)1 << 32), "snf_mxfp4_dequantize: %d x %d is too large for one launch", M, K);
     if (mx_aligned(out, 16) && ((int64_t)K * (int64_t)sizeof(T)) % 16 == 0)
         k_mxfp4_dequantize<T, true><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(codes, scales, M, K, chunks, out);
     else
@@ -311,7 +311,7 @@ static int mx_linear_t(const uint8_t* a, const uint8_t* as, const uint8_t* w, co
                        int act, T* y, hipStream_t st) {
     constexpr int BM = 128, BN = 128;
     const int chunks = ceil_div(K, 256), rts = ceil_div(M, BM), cts = ceil_div(N, BN);
-    SNF_REQUIRE((int64_t)rts * cts < ((int64_t)1 << 30), "snf_mxfp4_linear: %d x %d is too large for one launch", M, N);
+    SNF_REQUIRE(((int64_t)rts * cts + 8) * 256 < ((int64_t)1 << 32), "snf_mxfp4_linear: %d x %d is too large for one launch", M, N);
     const int per = (rts * cts + 7) / 8;
     k_mxfp4_linear<BM, BN, T><<<dim3(8 * per), dim3(256), 2 * 8 * (BM + BN) * 16, st>>>(a, as, w, ws, bias, M, N, chunks, act, y, rts, cts);
     SNF_LAUNCH_CHECK("snf_mxfp4_linear");

@@ -31,3 +31,18 @@ class MSELoss(torch.nn.Module):
         if pred.requires_grad or not target.requires_grad:
             return ops.mse_loss(pred, target)
         return ops.mse_loss(target, pred)
+
+
+class TopLogitsDistillLoss(torch.nn.Module):
+    """weight * T^2 KL(teacher || student) from the teacher's top logits (`ops.top_logits`), mean over the rows that have a target.
+    with_rest: the mass of the logits that the teacher's list leaves out is one class of its own; otherwise the teacher's
+    probabilities are those of its list alone.  The teacher's temperature must be this one where `with_rest` is on."""
+
+    def __init__(self, temperature: float = 1.0, weight: float = 1.0, with_rest: bool = True):
+        super().__init__()
+        self.temperature, self.weight, self.with_rest = temperature, weight, with_rest
+
+    def forward(self, student: torch.Tensor, teacher) -> torch.Tensor:
+        ids, logits, rest = teacher
+        return ops.top_logits_distill_loss(student, ids, logits, rest=rest if self.with_rest else None, temperature=self.temperature,
+                                           weight=self.weight)

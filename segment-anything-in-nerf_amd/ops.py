@@ -27,6 +27,7 @@ from . import _lib
 from ._opcore import *  # noqa: F401,F403
 from ._opcore import (_FN, _L, _TIMING, _chk, _has_gpu, _launch, _linear_fwd_ws, _p, _stream)  # noqa: F401
 from .ops_data import *  # noqa: F401,F403
+from .ops_distill import *  # noqa: F401,F403
 from .ops_losses import *  # noqa: F401,F403
 from .ops_losses import _Distortion, _Interlevel, _RowMSELoss  # noqa: F401
 from .ops_optim import *  # noqa: F401,F403

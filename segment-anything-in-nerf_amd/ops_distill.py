@@ -1,0 +1,152 @@
+"""A teacher's top logits and the distillation loss that reads them (csrc/distill.hip); `samnerf_amd.ops` re-exports everything here."""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ._opcore import DTYPE_CODE, _dev, _L, _launch, _p, _rows, _stream_on
+
+__all__ = ["TopLogits", "top_logits", "top_logits_distill_loss", "TOP_LOGITS_MAX_K", "TOP_LOGITS_MAX_V"]
+
+TOP_LOGITS_MAX_K = 256
+TOP_LOGITS_MAX_V = 1000000  # SNF_TOP_MAX_V
+
+_REDUCTIONS = ("mean", "sum", "none")
+
+
+class TopLogits(NamedTuple):
+    """What a teacher's answer is stored as: ids [..., k] int32 and logits [..., k], largest first, and rest [...] float32, the log-sum-exp
+    of logit / temperature over all the other places (-inf where there are none)."""
+    ids: torch.Tensor
+    logits: torch.Tensor
+    rest: torch.Tensor
+
+
+def _temperature(t) -> float:
+    t = float(t)
+    if not (t > 0.0 and math.isfinite(t)):
+        raise ValueError(f"temperature must be positive and finite, got {t}")
+    return t
+
+
+def _logits(t, name: str) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype not in DTYPE_CODE:
+        raise TypeError(f"{name}: float32, bfloat16 or float16 expected, got {getattr(t, 'dtype', type(t))}")
+    if t.dim() < 1 or not 1 <= t.shape[-1] <= TOP_LOGITS_MAX_V:
+        raise ValueError(f"{name}: rows of 1 to {TOP_LOGITS_MAX_V} logits expected, got {tuple(t.shape)}")
+
+
+def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
+    return torch.empty((nbytes // 8,), device=device, dtype=torch.int64) if nbytes else None
+
+
+@torch.no_grad()
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    """The k largest of logits [..., V] with their places and the log-sum-exp of logits / temperature over all other places.  Equal logits
+    come in the order of their places; a NaN counts as larger than everything.  k <= min(V, 256)."""
+    _logits(logits, "logits")
+    V, k = int(logits.shape[-1]), int(k)
+    if not 1 <= k <= min(V, TOP_LOGITS_MAX_K):
+        raise ValueError(f"top_logits: k={k} is not in 1 .. {min(V, TOP_LOGITS_MAX_K)}")
+    t = _temperature(temperature)
+    dev = _dev(logits, "logits")
+    lead = tuple(logits.shape[:-1])
+    ids = torch.empty(lead + (k,), device=dev, dtype=torch.int32)
+    vals = torch.empty(lead + (k,), device=dev, dtype=logits.dtype)
+    rest = torch.empty(lead, device=dev, dtype=torch.float32)
+    R = rest.numel()
+    if R:
+        x, ld = _rows(logits.unsqueeze(0) if logits.dim() == 1 else logits)
+        code = DTYPE_CODE[x.dtype]
+        nbytes = int(_L().snf_top_logits_workspace_bytes(R, V, k, code))
+        ws = _workspace(nbytes, dev)
+        _launch("snf_top_logits", _p(x), code, R, V, ld, k, t, _p(ids), _p(vals), _p(rest), _p(ws), nbytes, _stream_on(dev),
+                units=float(R * V * x.element_size()))
+    return TopLogits(ids, vals, rest)
+
+
+def _saved_parts(saved: torch.Tensor, R: int):
+    return saved[:4 * R], saved[4 * R:5 * R], saved[5 * R:]
+
+
+class _TopDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, student, ids, logits, rest, temperature: float, weight: float, reduction: str):
+        dev = student.device
+        V, K = int(student.shape[-1]), int(ids.shape[-1])
+        lead = tuple(student.shape[:-1])
+        z, ld = _rows(student.unsqueeze(0) if student.dim() == 1 else student)
+        ids, logits = ids.contiguous(), logits.contiguous()
+        rest = rest.contiguous() if rest is not None else None
+        R = z.shape[0]
+        code, st = DTYPE_CODE[z.dtype], _stream_on(dev)
+        rows = torch.empty(lead, device=dev, dtype=torch.float32)
+        saved = torch.empty((R * (5 + K),), device=dev, dtype=torch.float32)  # stats [R, 4], counted [R], p [R, K]
+        stats, counted, p = _saved_parts(saved, R)
+        if R:
+            nbytes = int(_L().snf_top_distill_workspace_bytes(R, V, code))
+            ws = _workspace(nbytes, dev)
+            _launch("snf_top_distill_fwd", _p(z), code, R, V, ld, _p(ids), int(ids.dtype == torch.int64), _p(logits),
+                    DTYPE_CODE[logits.dtype], _p(rest), K, temperature, weight, _p(rows), _p(counted), _p(stats), _p(p), _p(ws), nbytes, st,
+                    units=float(R * V * z.element_size()))
+        loss, divisor = rows, None
+        if reduction != "none":
+            loss, divisor = (torch.empty((), device=dev, dtype=torch.float32) for _ in range(2))
+            _launch("snf_top_distill_mean", _p(rows), _p(counted), R, int(reduction == "mean"), _p(loss), _p(divisor), st)
+        ctx.args = (tuple(student.shape), R, V, ld, K, temperature, weight, reduction)
+        ctx.save_for_backward(z, ids, saved, divisor)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        z, ids, saved, divisor = ctx.saved_tensors
+        shape, R, V, ld, K, temperature, weight, reduction = ctx.args
+        if not ctx.needs_input_grad[0]:
+            return (None,) * 7
+        dz = torch.empty(shape, device=z.device, dtype=z.dtype)
+        if R:
+            g = g.to(torch.float32).contiguous()
+            stats, counted, p = _saved_parts(saved, R)
+            _launch("snf_top_distill_bwd", _p(z), DTYPE_CODE[z.dtype], R, V, ld, _p(ids), int(ids.dtype == torch.int64), K, temperature,
+                    weight, _p(g), int(reduction == "none"), _p(divisor), _p(counted), _p(stats), _p(p), _p(dz), _stream_on(z.device),
+                    units=float(2 * R * V * z.element_size()))
+        return dz, None, None, None, None, None, None
+
+
+def top_logits_distill_loss(student: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor, rest: Optional[torch.Tensor] = None,
+                            temperature: float = 1.0, weight: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+    """weight * T^2 KL(teacher || student) from a teacher's top logits, with the student's gradient.
+
+    student [..., V] logits; ids [..., K] (int32 / int64; a negative id is no entry) and logits [..., K] as `top_logits` returns them (any
+    float type).  With rest [...] (float32, `top_logits` at the same temperature) the mass that the list leaves out is one class of its own,
+    against the student's mass on all places that the ids do not name; without it the teacher's probabilities sum to 1 over the list.
+    reduction "mean": over the rows with a target (a row without entries, or whose teacher has no mass, has none; no such row: 0); "sum";
+    "none": [...] float32.  An id named twice counts twice for the teacher; an id >= V makes its row NaN.  The teacher's tensors get no
+    gradient.  K <= 256."""
+    _logits(student, "student")
+    _logits(logits, "logits")
+    t = _temperature(temperature)
+    lead = tuple(student.shape[:-1])
+    if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"ids: int32 or int64 expected, got {getattr(ids, 'dtype', type(ids))}")
+    if ids.dim() != student.dim() or tuple(ids.shape[:-1]) != lead or not 1 <= ids.shape[-1] <= TOP_LOGITS_MAX_K:
+        raise ValueError(f"ids: {lead} rows of 1 to {TOP_LOGITS_MAX_K} expected, got {tuple(ids.shape)}")
+    if logits.shape != ids.shape:
+        raise ValueError(f"logits: {tuple(ids.shape)} expected, got {tuple(logits.shape)}")
+    if rest is not None:
+        if not isinstance(rest, torch.Tensor) or rest.dtype != torch.float32:
+            raise TypeError(f"rest: float32 expected, got {getattr(rest, 'dtype', type(rest))}")
+        if tuple(rest.shape) != lead:
+            raise ValueError(f"rest: {lead} expected, got {tuple(rest.shape)}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction: one of {_REDUCTIONS} expected, got {reduction!r}")
+    weight = float(weight)
+    dev = _dev(student, "student")
+    for name, other in (("ids", ids), ("logits", logits), ("rest", rest)):
+        if other is not None:
+            _dev(other, name, dev)
+    return _TopDistill.apply(student, ids, logits.detach(), rest.detach() if rest is not None else None, t, weight, reduction)
