@@ -67,11 +67,33 @@ struct TdMaxOp { __device__ static float op(float a, float b) { return td_max(a,
 struct TdSumOp { __device__ static float op(float a, float b) { return a + b; } };
 struct TdCountOp { __device__ static int op(int a, int b) { return a + b; } };
 
+template <int CTRL, typename V>
+__device__ __forceinline__ V td_dpp(V v) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+// over 8 neighbouring lanes / over the wave, in every lane, without LDS: lane swaps inside a quad, mirrored halves and rows of 16 lanes,
+// then rows and halves of the wave exchanged
+template <typename OP, typename V>
+__device__ __forceinline__ V td_reduce8(V v) {
+    v = OP::op(v, td_dpp<0xB1>(v));   // quad: 1 0 3 2
+    v = OP::op(v, td_dpp<0x4E>(v));   // quad: 2 3 0 1
+    return OP::op(v, td_dpp<0x141>(v));  // 8 lanes mirrored
+}
+template <typename OP, typename V>
+__device__ __forceinline__ V td_reduce_wave(V v) {
+    v = td_reduce8<OP>(v);
+    v = OP::op(v, td_dpp<0x140>(v));  // 16 lanes mirrored
+    const unsigned a = __builtin_bit_cast(unsigned, v);
+    const auto r16 = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    v = OP::op(__builtin_bit_cast(V, (unsigned)r16[0]), __builtin_bit_cast(V, (unsigned)r16[1]));
+    const unsigned b = __builtin_bit_cast(unsigned, v);
+    const auto r32 = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return OP::op(__builtin_bit_cast(V, (unsigned)r32[0]), __builtin_bit_cast(V, (unsigned)r32[1]));
+}
 // the same value in every thread of the workgroup; `s` is scratch of one word per wave, free again after the call
 template <int THREADS, typename OP, typename V>
 __device__ __forceinline__ V td_reduce(V v, V* s) {
-#pragma unroll
-    for (int d = WAVE / 2; d > 0; d >>= 1) v = OP::op(v, __shfl_xor(v, d, WAVE));
+    v = td_reduce_wave<OP>(v);
     if constexpr (THREADS > WAVE) {
         if (lane_id() == 0) s[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -106,21 +128,26 @@ struct TdPart {
             if (v < granules) r[j] = g[v];
         }
         // the granules at the two ends
-        if (threadIdx.x == 0)
-            for (int e = 0; e < shift; ++e) td_clear<T>(r[0], e);
-        const int last = granules - 1, over = granules * E - shift - n;
+        const int last = granules - 1;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (j * THREADS + (int)threadIdx.x == last)
-                for (int e = E - over; e < E; ++e) td_clear<T>(r[j], e);
+        for (int j = 0; j < NV; ++j) {
+            const int v = j * THREADS + (int)threadIdx.x;
+            if (v == 0 || v == last) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (!inside(place(j, e))) td_clear<T>(r[j], e);
+            }
+        }
     }
     __device__ __forceinline__ int place(int j, int e) const { return (j * THREADS + (int)threadIdx.x) * E + e - shift; }
     __device__ __forceinline__ bool inside(int place) const { return (unsigned)place < (unsigned)len; }
+    // (the empty asm keeps the unpacked values of one pass from staying in registers for the next)
     template <typename F>
-    __device__ __forceinline__ void each(F f) const {
+    __device__ __forceinline__ void each(F f) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             float x[E];
+            asm volatile("" : "+v"(r[j].x), "+v"(r[j].y), "+v"(r[j].z), "+v"(r[j].w));
             td_unpack<T>(r[j], x);
 #pragma unroll
             for (int e = 0; e < E; ++e) f(x[e], j, e);
@@ -131,209 +158,336 @@ struct TdPart {
 // =================================================================================================================================
 // top logits
 // =================================================================================================================================
-// One pass: (1) every thread's largest element; the k-th largest of G >= k group maxima is a bound that at least k elements reach and few
-// others do (G = 2 k groups: about 0.7 x 2 k of them for values in random order); (2) what reaches the bound goes to LDS as 64-bit keys
-// (value, place: all different, so ranks do not depend on the order of arrival), a key's rank is the number of larger keys; (3) the sum
-// over the rest refers to the largest logit of the rest, so that it keeps its digits however far below the top it lies.
-// Rows with a NaN and rows where more than TD_CAND elements reach the bound (long runs of equal logits) take the exact way: bisection of
-// the k-th key over its bits, then of the places among its equals.
+// A bound first: of G >= k disjoint sets of elements take the maxima; at least k elements reach the k-th largest of them, and few others
+// do (G = 2 k sets of values in random order: about 1.4 k elements).  What reaches the bound goes to LDS as 64-bit keys (value, place: all
+// different, so the order of arrival plays no part), and a key's rank is the number of larger keys.  The log-sum-exp of the rest refers to
+// the largest logit of the rest, so that it keeps its digits however far below the top it lies; it is never a difference.
+//   short rows (TD_SHAPES): the row in the registers of one workgroup, the sets are threads: one launch, one read.
+//   long rows: k_top_groups streams them -- any number of workgroups a row, nothing exchanged between waves -- and leaves the maximum and
+//     the sum of exponentials of every 128 bytes; k_top_select, one workgroup a row, finds the bound among the maxima and reads again only
+//     the groups that reach it (about 1.4 k of them: 9 % of a row of 65536 bf16 at k = 64; the groups' results are 6 %).
+// Rows with a NaN and rows where more than TD_CAND elements reach the bound (long runs of equal logits) take the exact way, from memory:
+// bisection of the k-th key over its bits, then of the places among its equals.
 constexpr int TD_CAND = 1024;
+constexpr int TD_GROUP = 8;  // 16-byte granules of a group (td_reduce8)
+
+template <int THREADS>
+struct TdSelect {
+    static constexpr int CAND = THREADS == 64 ? 256 : TD_CAND;
+    alignas(16) uint64_t key[CAND + 8];  // (filled up with zeros to a multiple of 8: a zero is below every key)
+    uint64_t sorted[CAND];
+    alignas(16) float set[THREADS];
+    float red[THREADS / WAVE];
+    uint32_t bound;
+    int n;
+};
+
+// the k-th largest of the sets' maxima; a set is THREADS / sets neighbouring threads (a power of two, at most 16), none has a NaN
+template <int THREADS>
+__device__ __forceinline__ float td_bound(TdSelect<THREADS>& s, float own, int k, int sets) {
+    const int per = THREADS / sets;
+    if (per >= 2) own = td_max(own, td_dpp<0xB1>(own));
+    if (per >= 4) own = td_max(own, td_dpp<0x4E>(own));
+    if (per >= 8) own = td_max(own, td_dpp<0x141>(own));
+    if (per >= 16) own = td_max(own, td_dpp<0x140>(own));
+    if ((int)threadIdx.x % per == 0) s.set[threadIdx.x / per] = own;
+    __syncthreads();
+    if ((int)threadIdx.x < sets) {
+        const float mine = s.set[threadIdx.x];
+        int ge = 0;
+#pragma unroll 8
+        for (int i = 0; i < sets / 4; ++i) {
+            const float4 f = reinterpret_cast<const float4*>(s.set)[i];
+            ge += (f.x >= mine) + (f.y >= mine) + (f.z >= mine) + (f.w >= mine);
+        }
+        if (ge >= k) atomicMax(&s.bound, td_key(mine));
+    }
+    __syncthreads();
+    return td_value(s.bound);
+}
+
+// keys of s.n <= CAND candidates in order; the first k leave
+template <int THREADS, typename T>
+__device__ __forceinline__ void td_rank(TdSelect<THREADS>& s, int k, int32_t* __restrict__ ids, T* __restrict__ logits) {
+    const int n = s.n;
+    if (threadIdx.x < 8) s.key[n + threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        const uint64_t mine = s.key[i];
+        int rank = 0;
+        for (int j = 0; j < n; j += 8) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(s.key + j + 2 * q);
+                rank += (two.x > mine) + (two.y > mine);
+            }
+        }
+        s.sorted[rank] = mine;
+        if (rank < k) {
+            ids[rank] = (int32_t)~(uint32_t)mine;
+            logits[rank] = (T)td_value((uint32_t)(mine >> 32));
+        }
+    }
+    __syncthreads();
+}
+
+// the elements of a row from memory
+template <typename T, int THREADS, typename F>
+__device__ __forceinline__ void td_scan(const T* p, int len, F f) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int shift = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+    const uint4* g = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
+    const int granules = (shift + len + E - 1) / E;
+#pragma unroll 1
+    for (int v = (int)threadIdx.x; v < granules; v += THREADS) {
+        float x[E];
+        td_unpack<T>(g[v], x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int at = v * E + e - shift;
+            if ((unsigned)at < (unsigned)len) f(x[e], at);
+        }
+    }
+}
+
+__device__ __forceinline__ float td_lse(float m, float sum, float temperature) {
+    return m == INFINITY || m == TD_NINF ? m : m / temperature + logf(sum);
+}
+
+// the exact way; returns the rest's log-sum-exp
+template <typename T, int THREADS>
+__device__ __noinline__ float td_select_exact(TdSelect<THREADS>& s, const T* src, int V, int k, float temperature, int32_t* ids, T* logits) {
+    const float c = TD_LOG2E / temperature;
+    auto count = [&](auto pred) {
+        int n = 0;
+        td_scan<T, THREADS>(src, V, [&](float v, int p) { n += pred(td_key(v), p); });
+        return td_reduce<THREADS, TdCountOp>(n, reinterpret_cast<int*>(s.red));
+    };
+    uint32_t kth = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t t = kth | 1u << bit;
+        if (count([&](uint32_t key, int) { return key >= t; }) >= k) kth = t;
+    }
+    const int need = k - count([&](uint32_t key, int) { return key > kth; });
+    const int equal = count([&](uint32_t key, int) { return key == kth; });
+    int cut = V;  // the smallest place with `need` equals before it
+    for (int lo = 0; need < equal && lo < cut;) {
+        const int mid = (lo + cut) >> 1;
+        if (count([&](uint32_t key, int p) { return key == kth && p < mid; }) >= need) cut = mid;
+        else lo = mid + 1;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    td_scan<T, THREADS>(src, V, [&](float v, int p) {
+        const uint32_t key = td_key(v);
+        if (key > kth || (key == kth && p < cut)) s.key[atomicAdd(&s.n, 1)] = (uint64_t)key << 32 | (uint32_t)~p;
+    });
+    __syncthreads();
+    td_rank<THREADS>(s, k, ids, logits);
+    float m = equal > need ? td_value(kth) : TD_NINF, sum = 0.f;
+    if (equal == need) {
+        td_scan<T, THREADS>(src, V, [&](float v, int) { if (td_key(v) < kth) m = td_max(m, v); });
+        m = td_reduce<THREADS, TdMaxOp>(m, s.red);
+    }
+    td_scan<T, THREADS>(src, V, [&](float v, int) { if (td_key(v) < kth) sum += td_term(v, m, c); });
+    sum = td_reduce<THREADS, TdSumOp>(sum, s.red) + (float)(equal - need);
+    return td_lse(m, sum, temperature);
+}
 
 template <typename T, int THREADS, int NV>
-__global__ __launch_bounds__(THREADS) void k_top_logits(const T* __restrict__ x, int V, int64_t ld, int k, int groups, float temperature,
-                                                        int parts, int part_len, int32_t* __restrict__ ids, T* __restrict__ logits,
-                                                        float* __restrict__ rest, uint64_t* __restrict__ part_keys,
-                                                        float2* __restrict__ part_rest) {
-    constexpr int CAND = THREADS == 64 ? 256 : TD_CAND;
-    __shared__ uint64_t s_key[CAND];
-    __shared__ float s_group[THREADS];
-    __shared__ float s_red[THREADS / WAVE];
-    __shared__ uint32_t s_bound;
-    __shared__ int s_n, s_equal;
-    __shared__ uint64_t s_kth, s_next;
-    const int row = (int)(blockIdx.x / (unsigned)parts), part = (int)(blockIdx.x % (unsigned)parts);
-    const int p0 = part * part_len, len = min(part_len, V - p0);
+__global__ __launch_bounds__(THREADS) void k_top_logits(const T* __restrict__ x, int V, int64_t ld, int k, int sets, float temperature,
+                                                        int32_t* __restrict__ ids, T* __restrict__ logits, float* __restrict__ rest) {
+    using Sel = TdSelect<THREADS>;
+    __shared__ Sel s;
+    const int64_t row = blockIdx.x;
+    ids += row * k;
+    logits += row * k;
+    const T* src = x + row * ld;
     TdPart<T, THREADS, NV> reg;
-    reg.load(x + (int64_t)row * ld + p0, len);
-    const int kk = min(k, len);
+    reg.load(src, V);
     const float c = TD_LOG2E / temperature;
-    if (threadIdx.x == 0) { s_bound = 0; s_n = 0; s_equal = 0; s_next = 0; }
-
+    if (threadIdx.x == 0) { s.bound = 0; s.n = 0; }
     float own = TD_NINF;
     reg.each([&](float v, int, int) { own = td_max(own, v); });
-    const float top = td_reduce<THREADS, TdMaxOp>(own, s_red);
-    bool slow = top != top;
-    if (!slow) {
-        // groups of THREADS / groups neighbouring threads (a power of two, at most a wave)
-        const int gs = THREADS / groups;
-        float gm = own;
-        for (int d = 1; d < gs; d <<= 1) gm = td_max(gm, __shfl_xor(gm, d, WAVE));
-        if ((int)threadIdx.x % gs == 0) s_group[threadIdx.x / gs] = gm;
-        __syncthreads();
-        if ((int)threadIdx.x < groups) {
-            const float mine = s_group[threadIdx.x];
-            int ge = 0;
-            for (int i = 0; i < groups; ++i) ge += s_group[i] >= mine;
-            if (ge >= kk) atomicMax(&s_bound, td_key(mine));
-        }
-        __syncthreads();
-        const float bound = td_value(s_bound);
-        if (own >= bound) {
+    const float top = td_reduce<THREADS, TdMaxOp>(own, s.red);
+    float bound = 0.f;
+    bool exact = top != top;
+    if (!exact) {
+        bound = td_bound<THREADS>(s, own, k, sets);
+        if (own >= bound)
             reg.each([&](float v, int j, int e) {
                 if (v >= bound) {
                     const int p = reg.place(j, e);
                     if (reg.inside(p)) {
-                        const int at = atomicAdd(&s_n, 1);
-                        if (at < CAND) s_key[at] = (uint64_t)td_key(v) << 32 | (uint32_t)~(p0 + p);
+                        const int at = atomicAdd(&s.n, 1);
+                        if (at < Sel::CAND) s.key[at] = (uint64_t)td_key(v) << 32 | (uint32_t)~p;
                     }
                 }
             });
-        }
         __syncthreads();
-        slow = s_n > CAND;
+        exact = s.n > Sel::CAND;
     }
-    uint32_t kth_key = 0;
-    int equal_left = 0;  // (slow) elements of the rest that equal the k-th
-    if (slow) {
-        int* s_redi = reinterpret_cast<int*>(s_red);
-        auto count = [&](auto pred) {
-            int n = 0;
-            reg.each([&](float v, int j, int e) {
-                const int p = reg.place(j, e);
-                n += reg.inside(p) && pred(td_key(v), p);
-            });
-            return td_reduce<THREADS, TdCountOp>(n, s_redi);
-        };
-        uint32_t v = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t t = v | 1u << bit;
-            if (count([&](uint32_t key, int) { return key >= t; }) >= kk) v = t;
-        }
-        const int need = kk - count([&](uint32_t key, int) { return key > v; });
-        const int equal = count([&](uint32_t key, int) { return key == v; });
-        int cut = len;  // the smallest with `need` equals before it
-        if (need < equal) {
-            int lo = 0;
-            while (lo < cut) {
-                const int mid = (lo + cut) >> 1;
-                if (count([&](uint32_t key, int p) { return key == v && p < mid; }) >= need) cut = mid;
-                else lo = mid + 1;
-            }
-        }
-        equal_left = equal - need;
-        kth_key = v;
-        __syncthreads();
-        if (threadIdx.x == 0) s_n = 0;
-        __syncthreads();
-        reg.each([&](float f, int j, int e) {
-            const int p = reg.place(j, e);
-            const uint32_t key = td_key(f);
-            if (reg.inside(p) && (key > v || (key == v && p < cut))) s_key[atomicAdd(&s_n, 1)] = (uint64_t)key << 32 | (uint32_t)~(p0 + p);
-        });
-        __syncthreads();
+    if (exact) {
+        const float r = td_select_exact<T, THREADS>(s, src, V, k, temperature, ids, logits);
+        if (threadIdx.x == 0) rest[row] = r;
+        return;
     }
-    const int n = s_n;  // kk <= n <= CAND
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-        const uint64_t mine = s_key[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += s_key[j] > mine;
-        if (rank < kk) {
-            if (parts == 1) {
-                ids[(int64_t)row * k + rank] = (int32_t)~(uint32_t)mine;
-                logits[(int64_t)row * k + rank] = (T)td_value((uint32_t)(mine >> 32));
-            } else {
-                part_keys[((int64_t)row * parts + part) * k + rank] = mine;
-            }
-            if (rank == kk - 1) s_kth = mine;
-        } else if (rank == kk) {
-            s_next = mine;
-        }
-    }
-    if (parts > 1)
-        for (int i = kk + threadIdx.x; i < k; i += THREADS) part_keys[((int64_t)row * parts + part) * k + i] = 0;  // a short part
-    __syncthreads();
+    td_rank<THREADS>(s, k, ids, logits);
+    const int n = s.n;
     float m, sum = 0.f;
-    if (!slow) {
-        const float kth = td_value((uint32_t)(s_kth >> 32));
-        if (n > kk) {
-            for (int i = threadIdx.x; i < n; i += THREADS)  // the candidates of the rest that equal the k-th
-                if ((uint32_t)(s_key[i] >> 32) == (uint32_t)(s_kth >> 32) && s_key[i] < s_kth) atomicAdd(&s_equal, 1);
-            m = td_value((uint32_t)(s_next >> 32));
-            __syncthreads();
-            equal_left = s_equal;
-        } else {
-            m = TD_NINF;
-            reg.each([&](float v, int, int) { if (v < kth) m = td_max(m, v); });
-            m = td_reduce<THREADS, TdMaxOp>(m, s_red);
-        }
-        if (m > TD_NINF)
-            reg.each([&](float v, int, int) { sum += v < kth ? td_exp2((v - m) * c) : 0.f; });
+    if (n > k) {
+        m = td_value((uint32_t)(s.sorted[k] >> 32));
     } else {
-        m = equal_left > 0 ? td_value(kth_key) : TD_NINF;
-        if (equal_left == 0) {
-            reg.each([&](float v, int, int) { if (td_key(v) < kth_key) m = td_max(m, v); });
-            m = td_reduce<THREADS, TdMaxOp>(m, s_red);
-        }
-        if (m != TD_NINF)
-            reg.each([&](float v, int, int) { sum += td_key(v) < kth_key ? td_term(v, m, c) : 0.f; });
+        m = TD_NINF;
+        reg.each([&](float v, int, int) { if (v < bound) m = td_max(m, v); });
+        m = td_reduce<THREADS, TdMaxOp>(m, s.red);
     }
-    sum = td_reduce<THREADS, TdSumOp>(sum, s_red) + (float)equal_left;
-    if (threadIdx.x == 0) {
-        if (m == TD_NINF) sum = 0.f;  // nothing left, or nothing but -inf
-        if (parts == 1) rest[row] = m == INFINITY || m == TD_NINF ? m : m / temperature + logf(sum);
-        else part_rest[(int64_t)row * parts + part] = make_float2(m, sum);
+    if (m > TD_NINF) reg.each([&](float v, int, int) { sum += v < bound ? td_exp2((v - m) * c) : 0.f; });
+    for (int i = k + threadIdx.x; i < n; i += THREADS) sum += td_term(td_value((uint32_t)(s.sorted[i] >> 32)), m, c);
+    sum = td_reduce<THREADS, TdSumOp>(sum, s.red);
+    if (threadIdx.x == 0) rest[row] = td_lse(m, sum, temperature);
+}
+
+// maximum and sum of exp((x - maximum) / T) of every group of TD_GROUP granules; a lane holds one granule of NV groups
+template <typename T, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS) void k_top_groups(const T* __restrict__ x, int V, int64_t ld, float temperature, int chunks, int groups,
+                                                        float2* __restrict__ out) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int64_t row = blockIdx.x / (unsigned)chunks;
+    const int g0 = (int)(blockIdx.x % (unsigned)chunks) * (THREADS * NV);  // the first granule
+    const T* src = x + row * ld;
+    const int shift = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
+    const uint4* g = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15);
+    const int last = (shift + V + E - 1) / E - 1;
+    const float c = TD_LOG2E / temperature;
+    uint4 r[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) r[j] = g[min(g0 + j * THREADS + (int)threadIdx.x, last)];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int v = g0 + j * THREADS + (int)threadIdx.x;
+        float f[E];
+        td_unpack<T>(r[j], f);
+        if (v == 0 || v >= last) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if ((unsigned)(v * E + e - shift) >= (unsigned)V) f[e] = TD_NINF;
+        }
+        float m = f[0];
+#pragma unroll
+        for (int e = 1; e < E; ++e) m = td_max(m, f[e]);
+        m = td_reduce8<TdMaxOp>(m);
+        const float ref = m == TD_NINF ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += td_exp2((f[e] - ref) * c);
+        sum = td_reduce8<TdSumOp>(sum);
+        if (v % TD_GROUP == 0 && v <= last) out[row * groups + v / TD_GROUP] = make_float2(m, sum);
     }
 }
 
-// the parts of a row joined: a key's rank is the sum of its places in the parts' sorted lists
-template <typename T>
-__global__ __launch_bounds__(256) void k_top_logits_join(int k, int parts, float temperature, const uint64_t* __restrict__ part_keys,
-                                                         const float2* __restrict__ part_rest, int32_t* __restrict__ ids,
-                                                         T* __restrict__ logits, float* __restrict__ rest) {
-    extern __shared__ uint64_t s_keys[];
-    __shared__ uint64_t s_next;
-    __shared__ float s_red[4];
-    const int row = blockIdx.x, n = parts * k;
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_top_select(const T* __restrict__ x, int V, int64_t ld, int k, int sets, float temperature, int groups,
+                                                        const float2* __restrict__ stats, int32_t* __restrict__ ids, T* __restrict__ logits,
+                                                        float* __restrict__ rest) {
+    using Sel = TdSelect<THREADS>;
+    constexpr int E = 16 / (int)sizeof(T);
+    __shared__ Sel s;
+    __shared__ int s_list[TD_CAND];  // the groups that reach the bound, in an order of their own (the sums below are always the same sums)
+    __shared__ int s_count[THREADS / WAVE];
+    const int64_t row = blockIdx.x;
+    ids += row * k;
+    logits += row * k;
+    stats += row * groups;
+    const T* src = x + row * ld;
+    const int shift = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
+    const uint4* g = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15);
+    const int granules = (shift + V + E - 1) / E, live = (granules + TD_GROUP - 1) / TD_GROUP;
     const float c = TD_LOG2E / temperature;
-    if (threadIdx.x == 0) s_next = 0;
-    for (int i = threadIdx.x; i < n; i += 256) s_keys[i] = part_keys[(int64_t)row * n + i];
-    __syncthreads();
-    uint32_t lost = 0;  // bit q: this thread's q-th key belongs to the rest (n <= 32 * 256)
-    for (int i = threadIdx.x, q = 0; i < n; i += 256, ++q) {
-        const uint64_t mine = s_keys[i];
-        if (mine == 0) continue;  // a short part's filling
-        int rank = 0;
-        for (int p = 0; p < parts; ++p) {
-            int lo = 0, hi = k;  // keys of part p above `mine`
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (s_keys[p * k + mid] > mine) lo = mid + 1; else hi = mid;
+    if (threadIdx.x == 0) { s.bound = 0; s.n = 0; }
+    float own = TD_NINF;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < live; i += THREADS) own = td_max(own, stats[i].x);
+    const float top = td_reduce<THREADS, TdMaxOp>(own, s.red);
+    bool exact = top != top;
+    float bound = 0.f, m = TD_NINF;  // m: the largest element below the bound
+    int found = 0;
+    if (!exact) {
+        bound = td_bound<THREADS>(s, own, k, sets);
+        int hits = 0;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < live; i += THREADS) {
+            const float gm = stats[i].x;
+            if (gm >= bound) ++hits;
+            else m = td_max(m, gm);
+        }
+        int incl = hits;
+#pragma unroll
+        for (int d = 1; d < WAVE; d <<= 1) {
+            const int t = __shfl_up(incl, d, WAVE);
+            if (lane_id() >= d) incl += t;
+        }
+        if (lane_id() == WAVE - 1) s_count[threadIdx.x >> 6] = incl;
+        __syncthreads();
+        int at = incl - hits;
+#pragma unroll
+        for (int w = 0; w < THREADS / WAVE; ++w) {
+            at += w < (int)(threadIdx.x >> 6) ? s_count[w] : 0;
+            found += s_count[w];
+        }
+        if (hits && found <= TD_CAND)
+            for (int i = threadIdx.x; i < live; i += THREADS)
+                if (stats[i].x >= bound) s_list[at++] = i;
+        __syncthreads();
+        exact = found > TD_CAND;
+    }
+    const int team = (int)threadIdx.x / TD_GROUP, member = (int)threadIdx.x % TD_GROUP;
+    auto sweep = [&](auto f) {
+#pragma unroll 4
+        for (int q = team; q < found; q += THREADS / TD_GROUP) {
+            const int v = s_list[q] * TD_GROUP + member;
+            if (v >= granules) continue;
+            float e_[E];
+            td_unpack<T>(g[v], e_);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if ((unsigned)(v * E + e - shift) < (unsigned)V) f(e_[e], v * E + e - shift);
+        }
+    };
+    if (!exact) {
+        sweep([&](float v, int p) {
+            if (v >= bound) {
+                const int at = atomicAdd(&s.n, 1);
+                if (at < Sel::CAND) s.key[at] = (uint64_t)td_key(v) << 32 | (uint32_t)~p;
+            } else {
+                m = td_max(m, v);
             }
-            rank += lo;
-        }
-        if (rank < k) {
-            ids[(int64_t)row * k + rank] = (int32_t)~(uint32_t)mine;
-            logits[(int64_t)row * k + rank] = (T)td_value((uint32_t)(mine >> 32));
-        } else {
-            lost |= 1u << q;
-            if (rank == k) s_next = mine;
-        }
+        });
+        __syncthreads();
+        exact = s.n > Sel::CAND;
     }
-    __syncthreads();
-    float m = s_next ? td_value((uint32_t)(s_next >> 32)) : TD_NINF;
-    for (int p = threadIdx.x; p < parts; p += 256) m = td_max(m, part_rest[(int64_t)row * parts + p].x);
-    m = td_reduce<256, TdMaxOp>(m, s_red);
+    if (exact) {
+        const float r = td_select_exact<T, THREADS>(s, src, V, k, temperature, ids, logits);
+        if (threadIdx.x == 0) rest[row] = r;
+        return;
+    }
+    td_rank<THREADS>(s, k, ids, logits);
+    const int n = s.n;
+    m = td_reduce<THREADS, TdMaxOp>(m, s.red);
+    if (n > k) m = td_value((uint32_t)(s.sorted[k] >> 32));
     float sum = 0.f;
-    if (m != TD_NINF) {
-        for (int i = threadIdx.x, q = 0; i < n; i += 256, ++q)
-            if (lost >> q & 1u) sum += td_term(td_value((uint32_t)(s_keys[i] >> 32)), m, c);
-        for (int p = threadIdx.x; p < parts; p += 256) {
-            const float2 pr = part_rest[(int64_t)row * parts + p];
-            sum += pr.y * td_term(pr.x, m, c);
+    if (m > TD_NINF) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < live; i += THREADS) {
+            const float2 st = stats[i];
+            if (st.x < bound) sum += st.y * td_term(st.x, m, c);
         }
+        sweep([&](float v, int) { if (v < bound) sum += td_term(v, m, c); });
     }
-    sum = td_reduce<256, TdSumOp>(sum, s_red);
-    if (threadIdx.x == 0) rest[row] = m == INFINITY || m == TD_NINF ? m : m / temperature + logf(sum);
+    for (int i = k + threadIdx.x; i < n; i += THREADS) sum += td_term(td_value((uint32_t)(s.sorted[i] >> 32)), m, c);
+    sum = td_reduce<THREADS, TdSumOp>(sum, s.red);
+    if (threadIdx.x == 0) rest[row] = td_lse(m, sum, temperature);
 }
 
 // =================================================================================================================================
@@ -399,8 +553,7 @@ __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V,
     }
     bad = __any(bad);
     any = __any(any) || bad;
-#pragma unroll
-    for (int d = WAVE / 2; d > 0; d >>= 1) tm = td_max(tm, __shfl_xor(tm, d, WAVE));
+    tm = td_reduce_wave<TdMaxOp>(tm);
     const float r = REST ? t.rest[row] : TD_NINF;
     if (REST) tm = td_max(tm, r);
     if (!any || (tm == TD_NINF && !bad)) {  // no target: no entry, or a teacher without any mass
@@ -420,7 +573,7 @@ __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V,
         pe[q] = id[q] >= 0 ? expf(tv[q]) : 0.f;
         ps += pe[q];
     }
-    ps = wave_sum(ps);
+    ps = td_reduce_wave<TdSumOp>(ps);
     const float re = REST ? expf(r - tm) : 0.f;
     ps += re;
     const float log_ps = logf(ps);
@@ -430,8 +583,7 @@ __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V,
         float nm = TD_NINF;
 #pragma unroll
         for (int q = 0; q < Q; ++q) nm = td_max(nm, zv[q]);
-#pragma unroll
-        for (int d = WAVE / 2; d > 0; d >>= 1) nm = td_max(nm, __shfl_xor(nm, d, WAVE));
+        nm = td_reduce_wave<TdMaxOp>(nm);
         m = td_max(m_r, nm);
         float sn = 0.f;
 #pragma unroll
@@ -442,12 +594,12 @@ __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V,
             for (int q2 = 0; q2 <= q; ++q2)
                 for (int l = 0; l < (q2 < q ? WAVE : WAVE - 1); ++l) {
                     if (q2 * WAVE + l >= t.K) break;
-                    const int other = __shfl((int)id[q2], l, WAVE);
+                    const int other = __builtin_amdgcn_readlane((int)id[q2], l);
                     if (q2 * WAVE + l < q * WAVE + lane && other == (int)id[q]) first = false;
                 }
             if (first) sn += td_term(zv[q], m, c);
         }
-        s = wave_sum(sn) + s_r * td_term(m_r, m, c);
+        s = td_reduce_wave<TdSumOp>(sn) + s_r * td_term(m_r, m, c);
     }
     const float log_s = logf(s);
     float loss = 0.f;
@@ -458,7 +610,7 @@ __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V,
         if (k < t.K) out.p[row * t.K + k] = p;
         if (id[q] >= 0 && (p > 0.f || p != p)) loss += p * ((tv[q] - log_ps) - ((zv[q] - m) / temperature - log_s));
     }
-    loss = wave_sum(loss);
+    loss = td_reduce_wave<TdSumOp>(loss);
     float f = 1.f / s, ref = m;
     if (REST) {
         const float pr = re / ps;
@@ -487,13 +639,16 @@ __global__ __launch_bounds__(THREADS) void k_top_distill_rows(const T* __restric
     const int part = (int)(blockIdx.x % (unsigned)parts);
     const int p0 = part * part_len, len = min(part_len, V - p0);
     const T* zrow = z + row * ld;
+    // (the ids are asked for before the row: loads come back in order)
+    int64_t first_id = -1;
+    if (REST && (int)threadIdx.x < t.K) first_id = td_id(t.ids, t.ids_wide, row * t.K + threadIdx.x);
     Part reg;
     reg.load(zrow + p0, len);
     if (REST) {  // the named places become -inf: one bit per place of the part, in the order of the registers
         for (int i = threadIdx.x; i < WORDS; i += THREADS) s_named[i] = 0;
         __syncthreads();
         for (int k = threadIdx.x; k < t.K; k += THREADS) {
-            const int64_t i = td_id(t.ids, t.ids_wide, row * t.K + k) - p0;
+            const int64_t i = (k < THREADS ? first_id : td_id(t.ids, t.ids_wide, row * t.K + k)) - p0;
             if (i >= 0 && i < len) atomicOr(&s_named[(i + reg.shift) >> 5], 1u << ((i + reg.shift) & 31));
         }
         __syncthreads();
@@ -528,13 +683,12 @@ __global__ __launch_bounds__(64) void k_top_distill_join(const T* __restrict__ z
     const float c = TD_LOG2E / temperature;
     float m = TD_NINF, s = 0.f;
     for (int p = lane_id(); p < parts; p += WAVE) m = td_max(m, part_ms[row * parts + p].x);
-#pragma unroll
-    for (int d = WAVE / 2; d > 0; d >>= 1) m = td_max(m, __shfl_xor(m, d, WAVE));
+    m = td_reduce_wave<TdMaxOp>(m);
     for (int p = lane_id(); p < parts; p += WAVE) {
         const float2 ms = part_ms[row * parts + p];
         s += ms.y * td_term(ms.x, m, c);
     }
-    s = wave_sum(s);
+    s = td_reduce_wave<TdSumOp>(s);
     td_finish_row<T, REST>(z + row * ld, V, row, t, temperature, scale, m, s, out);
 }
 
@@ -641,63 +795,74 @@ __global__ __launch_bounds__(256) void k_top_distill_bwd(const T* __restrict__ z
 // ---- launch shapes ----------------------------------------------------------------------------------------------------------------
 // shapes a row (or a part of it) is held in, smallest first: threads x 16-byte granules a thread
 struct TdShape { int threads, nv; };
-constexpr TdShape TD_SHAPES[] = {{64, 1}, {64, 4}, {256, 4}, {256, 16}, {512, 16}};
-constexpr int TD_NSHAPES = 5;
+constexpr TdShape TD_SHAPES[] = {{64, 1}, {64, 4}, {64, 8}, {256, 4}, {512, 4}};
+constexpr int td_capacity(int shape, int E) { return TD_SHAPES[shape].threads * TD_SHAPES[shape].nv * E - E; }
 
 struct TdPlan { int shape, parts, part_len; };
 
-// The smallest shape that holds a row; where that leaves most of the chip idle (fewer than 256 workgroups), smaller parts of a row per
-// workgroup and a join -- down to the wave of four granules, and to no more parts than `max_parts`.
-static TdPlan td_plan(int R, int V, int E, int min_threads, int max_parts) {
-    auto cap = [&](int s) { return TD_SHAPES[s].threads * TD_SHAPES[s].nv * E - E; };
+// Loss: the smallest wave that holds a row; long rows are dealt out in parts of 8 KB, a wave each (no barriers, and every wave's loads are
+// under way at once: 4096 x 65536 bf16 in 150 us with workgroups of 256 threads x 16 KB, 130 with waves), of 4 KB where that makes fewer
+// than 256 of them.
+static TdPlan td_rows_plan(int R, int V, int E) {
     int s = 0;
-    while (s + 1 < TD_NSHAPES && (cap(s) < V || TD_SHAPES[s].threads < min_threads)) ++s;
-    int parts = ceil_div(V, cap(s));
-    while (s > 1 && TD_SHAPES[s - 1].threads >= min_threads && (long long)R * parts < 256 && ceil_div(V, cap(s - 1)) <= max_parts) {
-        --s;
-        parts = ceil_div(V, cap(s));
-    }
-    return {s, parts, parts == 1 ? V : cap(s)};
+    while (s < 2 && td_capacity(s, E) < V) ++s;
+    if (s == 2 && (int64_t)R * ceil_div(V, td_capacity(s, E)) < 256) s = 1;
+    const int parts = ceil_div(V, td_capacity(s, E));
+    return {s, parts, parts == 1 ? V : td_capacity(s, E)};
 }
 
-static TdPlan td_top_plan(int R, int V, int k, int E) {
-    // 2 k threads where there are as many (the bound is the k-th of the groups' maxima); at most 1024 keys to join unless the row is
-    // longer than 1024 / k parts of the largest shape (V <= SNF_TOP_MAX_V: at most 32 parts, 8192 keys, 64 KB)
-    return td_plan(R, V, E, k <= 32 ? 64 : k <= 128 ? 256 : 512, 1024 / k);
+// Selection: the smallest shape that holds a row and has 2 k threads (sets for the bound; k for k > 256 / 2 threads of the largest), or -1:
+// a long row.
+static int td_top_shape(int V, int k, int E) {
+    if (k <= 32 && td_capacity(0, E) >= V) return 0;
+    if (k <= 32 && td_capacity(1, E) >= V) return 1;
+    if (k <= 128 && td_capacity(3, E) >= V) return 3;
+    if (k > 128 && td_capacity(4, E) >= V) return 4;
+    return -1;
 }
+// groups of a row, wherever it begins in a granule
+static int td_top_group_count(int V, int E) { return ceil_div((int64_t)V + E - 1, E * TD_GROUP); }
 
 template <typename T>
 static int td_top_t(const T* x, int R, int V, int64_t ld, int k, float temperature, int32_t* ids, T* logits, float* rest, void* ws,
                     hipStream_t st) {
-    const TdPlan pl = td_top_plan(R, V, k, 16 / (int)sizeof(T));
-    SNF_REQUIRE((int64_t)R * pl.parts * TD_SHAPES[pl.shape].threads < ((int64_t)1 << 32), "snf_top_logits: %d rows of %d are too many for one launch", R, V);
-    uint64_t* keys = (uint64_t*)ws;
-    float2* pr = (float2*)(keys + (size_t)R * pl.parts * k);
-    const int threads = TD_SHAPES[pl.shape].threads;
-    int groups = 32;
-    while (groups < 2 * k) groups *= 2;
-    if (groups > threads) groups = threads;
-    if (threads / groups > WAVE) groups = threads / WAVE;
-    const dim3 grid((unsigned)((int64_t)R * pl.parts));
+    constexpr int E = 16 / (int)sizeof(T);
+    const int shape = td_top_shape(V, k, E);
+    const int threads = shape >= 0 ? TD_SHAPES[shape].threads : k <= 128 ? 256 : 512;
+    SNF_REQUIRE((int64_t)R * threads < ((int64_t)1 << 32), "snf_top_logits: %d rows are too many for one launch", R);
+    int sets = 32;
+    while (sets < 2 * k) sets *= 2;
+    if (sets > threads) sets = threads;
 #define TD_GO(S_)                                                                                                                     \
     case S_:                                                                                                                          \
-        k_top_logits<T, TD_SHAPES[S_].threads, TD_SHAPES[S_].nv><<<grid, dim3(TD_SHAPES[S_].threads), 0, st>>>(                       \
-            x, V, ld, k, groups, temperature, pl.parts, pl.part_len, ids, logits, rest, keys, pr);                                    \
+        k_top_logits<T, TD_SHAPES[S_].threads, TD_SHAPES[S_].nv><<<dim3(R), dim3(threads), 0, st>>>(x, V, ld, k, sets, temperature, ids,  \
+                                                                                                    logits, rest);                    \
         break;
-    switch (pl.shape) { TD_GO(0) TD_GO(1) TD_GO(2) TD_GO(3) TD_GO(4) }
-#undef TD_GO
-    SNF_LAUNCH_CHECK("snf_top_logits");
-    if (pl.parts > 1) {
-        k_top_logits_join<T><<<dim3(R), dim3(256), (size_t)pl.parts * k * 8, st>>>(k, pl.parts, temperature, keys, pr, ids, logits, rest);
-        SNF_LAUNCH_CHECK("snf_top_logits (join)");
+    if (shape >= 0) {
+        switch (shape) { TD_GO(0) TD_GO(1) TD_GO(3) TD_GO(4) }
+        SNF_LAUNCH_CHECK("snf_top_logits");
+        return SNF_OK;
     }
+#undef TD_GO
+    const int groups = td_top_group_count(V, E), granules = groups * TD_GROUP;
+    // 16 KB a workgroup; 4 KB where that makes fewer than 1024 of them
+    const int64_t big = (int64_t)R * ceil_div(granules, 256 * 4);
+    const int per = big < 1024 ? 64 * 4 : 256 * 4, chunks = ceil_div(granules, per);
+    SNF_REQUIRE((int64_t)R * chunks * (per / 4) < ((int64_t)1 << 32), "snf_top_logits: %d rows of %d are too many for one launch", R, V);
+    const dim3 grid((unsigned)((int64_t)R * chunks));
+    if (per == 256) k_top_groups<T, 64, 4><<<grid, dim3(64), 0, st>>>(x, V, ld, temperature, chunks, groups, (float2*)ws);
+    else k_top_groups<T, 256, 4><<<grid, dim3(256), 0, st>>>(x, V, ld, temperature, chunks, groups, (float2*)ws);
+    SNF_LAUNCH_CHECK("snf_top_logits (groups)");
+    if (threads == 256) k_top_select<T, 256><<<dim3(R), dim3(256), 0, st>>>(x, V, ld, k, sets, temperature, groups, (const float2*)ws, ids, logits, rest);
+    else k_top_select<T, 512><<<dim3(R), dim3(512), 0, st>>>(x, V, ld, k, sets, temperature, groups, (const float2*)ws, ids, logits, rest);
+    SNF_LAUNCH_CHECK("snf_top_logits (select)");
     return SNF_OK;
 }
 
 template <typename T, bool REST>
 static int td_fwd_t(const T* z, int R, int V, int64_t ld, const TdTeacher& t, float temperature, float weight, const TdSaved& out, void* ws,
                     hipStream_t st) {
-    const TdPlan pl = td_plan(R, V, 16 / (int)sizeof(T), 64, 1 << 30);
+    const TdPlan pl = td_rows_plan(R, V, 16 / (int)sizeof(T));
     SNF_REQUIRE((int64_t)R * pl.parts * TD_SHAPES[pl.shape].threads < ((int64_t)1 << 32), "snf_top_distill_fwd: %d rows of %d are too many for one launch", R, V);
     const float scale = weight * temperature * temperature;
     const dim3 grid((unsigned)((int64_t)R * pl.parts));
@@ -706,7 +871,7 @@ static int td_fwd_t(const T* z, int R, int V, int64_t ld, const TdTeacher& t, fl
         k_top_distill_rows<T, REST, TD_SHAPES[S_].threads, TD_SHAPES[S_].nv><<<grid, dim3(TD_SHAPES[S_].threads), 0, st>>>(           \
             z, V, ld, t, temperature, scale, pl.parts, pl.part_len, out, (float2*)ws);                                                \
         break;
-    switch (pl.shape) { TD_GO(0) TD_GO(1) TD_GO(2) TD_GO(3) TD_GO(4) }
+    switch (pl.shape) { TD_GO(0) TD_GO(1) TD_GO(2) }
 #undef TD_GO
     SNF_LAUNCH_CHECK("snf_top_distill_fwd");
     if (pl.parts > 1) {
@@ -741,8 +906,8 @@ extern "C" {
 
 int64_t snf_top_logits_workspace_bytes(int R, int V, int k, int dtype) {
     if (R < 1 || V < 1 || k < 1 || k > snf::TD_MAX_K || k > V) return 0;
-    const snf::TdPlan pl = snf::td_top_plan(R, V, k, dtype == SNF_F32 ? 4 : 8);
-    return pl.parts == 1 ? 0 : (int64_t)R * pl.parts * (8 * (int64_t)k + 8);
+    const int E = dtype == SNF_F32 ? 4 : 8;
+    return snf::td_top_shape(V, k, E) >= 0 ? 0 : (int64_t)R * snf::td_top_group_count(V, E) * 8;
 }
 
 int snf_top_logits(const void* x, int dtype, int R, int V, int64_t ld, int k, float temperature, int32_t* ids, void* logits, float* rest,
@@ -766,7 +931,7 @@ int snf_top_logits(const void* x, int dtype, int R, int V, int64_t ld, int k, fl
 
 int64_t snf_top_distill_workspace_bytes(int R, int V, int dtype) {
     if (R < 1 || V < 1) return 0;
-    const snf::TdPlan pl = snf::td_plan(R, V, dtype == SNF_F32 ? 4 : 8, 64, 1 << 30);
+    const snf::TdPlan pl = snf::td_rows_plan(R, V, dtype == SNF_F32 ? 4 : 8);
     return pl.parts == 1 ? 0 : (int64_t)R * pl.parts * 8;
 }
 
