@@ -524,11 +524,11 @@ int snf_attention_planes_rp(const float* qkv, const float* rel_pos_h, const floa
  *   sum of q over the places that the row's ids do not name:
  *     rows[r] = weight T^2 ( sum_k p_k (log p_k - log q_ids_k) + p_rest (log p_rest - log q_rest) )
  *   without rest, p sums to 1 over the entries.  Rows without an entry, or whose teacher has no mass, are no targets: rows = counted = 0.
- *   An id >= V makes its row NaN.  stats [R, 4] (16-byte aligned) and p [R, K] are kept for the backward pass.  workspace:
+ *   An id >= V makes its row NaN.  stats [R, 4] (16-byte aligned) and p [R, K] are kept for the backward pass.  loss (or NULL) [1] = sum of
+ *   rows / divisor[0], divisor [1] = number of counted rows (at least 1) or, mean == 0, 1.  workspace:
  *   snf_top_distill_workspace_bytes(...) bytes, 8-byte aligned.
- * snf_top_distill_mean: loss[0] = sum of rows / divisor[0], divisor[0] = number of counted rows (at least 1) or, mean == 0, 1.
  * snf_top_distill_bwd: dz [R, V] contiguous of `dtype` = g weight T (q_v - sum_{k: ids_k = v} p_k - (v not named) p_rest q_v / q_rest),
- *   divided by divisor[0] where divisor (of snf_top_distill_mean) is given; g [1], or [R] where g_per_row.  Rows that are no
+ *   divided by divisor[0] where it is given; g [1], or [R] where g_per_row.  Rows that are no
  *   targets get zeros. */
 #define SNF_TOP_MAX_V 1000000
 int64_t snf_top_logits_workspace_bytes(int R, int V, int k, int dtype);
@@ -537,9 +537,7 @@ int snf_top_logits(const void* x, int dtype, int R, int V, int64_t ld, int k, fl
 int64_t snf_top_distill_workspace_bytes(int R, int V, int dtype);
 int snf_top_distill_fwd(const void* z, int dtype, int R, int V, int64_t ld, const void* ids, int ids_wide, const void* top, int top_dtype,
                         const float* rest, int K, float temperature, float weight, float* rows, float* counted, float* stats, float* p,
-                        void* workspace, int64_t workspace_bytes, snf_stream_t stream);
-int snf_top_distill_mean(const float* rows, const float* counted, int R, int mean, float* loss, float* divisor,
-                         snf_stream_t stream);
+                        int mean, float* loss, float* divisor, void* workspace, int64_t workspace_bytes, snf_stream_t stream);
 int snf_top_distill_bwd(const void* z, int dtype, int R, int V, int64_t ld, const void* ids, int ids_wide, int K, float temperature,
                         float weight, const float* g, int g_per_row, const float* divisor, const float* counted, const float* stats,
                         const float* p, void* dz, snf_stream_t stream);
@@ -553,11 +551,16 @@ int snf_top_distill_bwd(const void* z, int dtype, int R, int V, int64_t ld, cons
  *   8 c + 2 j + h (4-byte aligned).  The columns from K to 256 C hold zeros.
  * snf_mxfp4_quantize: x [M, K] of `dtype` with rows `ld` elements apart.  snf_mxfp4_dequantize: the values of the codes, out [M, K]
  *   contiguous.  snf_mxfp4_linear: y [M, N] of `dtype` = act(a w^T + bias), w quantised from [N, K], bias [N] fp32 or NULL, fp32 sums.
- *   Products below 2^-126 count as zero.  M = 0 is a call without work. */
+ *   Products below 2^-126 count as zero.  M = 0 is a call without work.
+ * snf_mxfp4_linear_rows: the same for up to SNF_MXFP4_ROWS rows x [M, K] of `dtype` (rows `ld` elements apart) that are quantised on the
+ *   way into the product: one launch.  The same result as snf_mxfp4_quantize followed by snf_mxfp4_linear. */
+#define SNF_MXFP4_ROWS 16
 int snf_mxfp4_quantize(const void* x, int dtype, int M, int K, int64_t ld, uint8_t* codes, uint8_t* scales, snf_stream_t stream);
 int snf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* out, int dtype, snf_stream_t stream);
 int snf_mxfp4_linear(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* w_codes, const uint8_t* w_scales, const float* bias,
                      int M, int K, int N, int act, void* y, int dtype, snf_stream_t stream);
+int snf_mxfp4_linear_rows(const void* x, int dtype, int64_t ld, const uint8_t* w_codes, const uint8_t* w_scales, const float* bias, int M,
+                          int K, int N, int act, void* y, int out_dtype, snf_stream_t stream);
 
 /* ---- the batch builder in front of the path (images, feature maps and cameras resident in HBM).
  * snf_pixel_indices: PixelSampler (patch == 1: u [B,3]) / PatchPixelSampler (u [B/patch^2,3]) .sample_method without a

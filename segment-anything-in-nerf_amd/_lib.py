@@ -157,12 +157,12 @@ SIGNATURES = {
     "snf_attention_planes": [P, P, I, I, I, I, I, F, P, P, P],
     "snf_attention_planes_rp": [P, P, P, I, I, I, I, I, F, P, P, P],
     "snf_top_logits": [P, I, I, I, c_int64, I, F, P, P, P, P, c_int64, P],
-    "snf_top_distill_fwd": [P, I, I, I, c_int64, P, I, P, I, P, I, F, F, P, P, P, P, P, c_int64, P],
-    "snf_top_distill_mean": [P, P, I, I, P, P, P],
+    "snf_top_distill_fwd": [P, I, I, I, c_int64, P, I, P, I, P, I, F, F, P, P, P, P, I, P, P, P, c_int64, P],
     "snf_top_distill_bwd": [P, I, I, I, c_int64, P, I, I, F, F, P, I, P, P, P, P, P, P],
     "snf_mxfp4_quantize": [P, I, I, I, c_int64, P, P, P],
     "snf_mxfp4_dequantize": [P, P, I, I, P, I, P],
     "snf_mxfp4_linear": [P, P, P, P, P, I, I, I, I, P, I, P],
+    "snf_mxfp4_linear_rows": [P, I, c_int64, P, P, P, I, I, I, I, P, I, P],
     "snf_pixel_indices": [P, I, I, I, I, I, P, P],
     "snf_generate_rays": [P, I, P, P, I, P, P, P, P, P],
     "snf_gather_nearest": [P, I, I, I, P, I, I, I, I, I, I, P, P],

@@ -881,6 +881,12 @@ static int td_fwd_t(const T* z, int R, int V, int64_t ld, const TdTeacher& t, fl
     return SNF_OK;
 }
 
+static int td_mean(const float* rows, const float* counted, int R, int mean, float* loss, float* divisor, hipStream_t st) {
+    k_top_distill_mean<<<dim3(1), dim3(1024), 0, st>>>(rows, counted, R, mean, loss, divisor);
+    SNF_LAUNCH_CHECK("snf_top_distill_fwd (mean)");
+    return SNF_OK;
+}
+
 template <typename T>
 static int td_bwd_t(const T* z, int R, int V, int64_t ld, const void* ids, int ids_wide, int K, float temperature, float weight,
                     const float* g, int g_per_row, const float* divisor, const float* counted, const float4* stats, const float* p, T* dz,
@@ -937,37 +943,26 @@ int64_t snf_top_distill_workspace_bytes(int R, int V, int dtype) {
 
 int snf_top_distill_fwd(const void* z, int dtype, int R, int V, int64_t ld, const void* ids, int ids_wide, const void* top, int top_dtype,
                         const float* rest, int K, float temperature, float weight, float* rows, float* counted, float* stats, float* p,
-                        void* workspace, int64_t workspace_bytes, snf_stream_t stream) {
+                        int mean, float* loss, float* divisor, void* workspace, int64_t workspace_bytes, snf_stream_t stream) {
     SNF_REQUIRE(R >= 0 && V >= 1 && V <= SNF_TOP_MAX_V, "snf_top_distill_fwd: bad sizes R=%d V=%d", R, V);
     SNF_REQUIRE(K >= 1 && K <= snf::TD_MAX_K, "snf_top_distill_fwd: K=%d is not in 1 .. %d", K, snf::TD_MAX_K);
     SNF_REQUIRE(temperature > 0.f && temperature < INFINITY, "snf_top_distill_fwd: temperature %g", (double)temperature);
     SNF_REQUIRE(dtype >= SNF_F32 && dtype <= SNF_F16 && top_dtype >= SNF_F32 && top_dtype <= SNF_F16, "snf_top_distill_fwd: unknown dtype");
-    if (R == 0) return SNF_OK;
+    SNF_REQUIRE(!loss || divisor, "snf_top_distill_fwd: null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    if (R == 0) return loss ? snf::td_mean(rows, counted, R, mean, loss, divisor, st) : SNF_OK;
     SNF_REQUIRE(z && ids && top && rows && counted && stats && p, "snf_top_distill_fwd: null pointer");
     SNF_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0, "snf_top_distill_fwd: stats is not aligned to 16 bytes");
     SNF_REQUIRE(ld >= V || R == 1, "snf_top_distill_fwd: rows of %d values overlap at stride %lld", V, (long long)ld);
     SNF_REQUIRE(workspace_bytes >= snf_top_distill_workspace_bytes(R, V, dtype) && (workspace_bytes == 0 || workspace),
                 "snf_top_distill_fwd: workspace of %lld bytes is too small", (long long)workspace_bytes);
-    hipStream_t st = (hipStream_t)stream;
     const snf::TdTeacher t{ids, top, rest, ids_wide, top_dtype, K};
     const snf::TdSaved out{rows, counted, (float4*)stats, p};
 #define TD_T(T_) (rest ? snf::td_fwd_t<T_, true>((const T_*)z, R, V, ld, t, temperature, weight, out, workspace, st)                  \
                        : snf::td_fwd_t<T_, false>((const T_*)z, R, V, ld, t, temperature, weight, out, workspace, st))
-    switch (dtype) {
-        case SNF_F32: return TD_T(float);
-        case SNF_BF16: return TD_T(__bf16);
-        default: return TD_T(_Float16);
-    }
+    const int rc = dtype == SNF_F32 ? TD_T(float) : dtype == SNF_BF16 ? TD_T(__bf16) : TD_T(_Float16);
 #undef TD_T
-}
-
-int snf_top_distill_mean(const float* rows, const float* counted, int R, int mean, float* loss, float* divisor,
-                         snf_stream_t stream) {
-    SNF_REQUIRE(R >= 0, "snf_top_distill_mean: bad size R=%d", R);
-    SNF_REQUIRE(loss && divisor && (R == 0 || (rows && counted)), "snf_top_distill_mean: null pointer");
-    snf::k_top_distill_mean<<<dim3(1), dim3(1024), 0, (hipStream_t)stream>>>(rows, counted, R, mean, loss, divisor);
-    SNF_LAUNCH_CHECK("snf_top_distill_mean");
-    return SNF_OK;
+    return rc != SNF_OK || !loss ? rc : snf::td_mean(rows, counted, R, mean, loss, divisor, st);
 }
 
 int snf_top_distill_bwd(const void* z, int dtype, int R, int V, int64_t ld, const void* ids, int ids_wide, int K, float temperature,

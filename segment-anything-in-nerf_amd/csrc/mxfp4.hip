@@ -278,6 +278,96 @@ __global__ __launch_bounds__(256) void k_mxfp4_linear(const uint8_t* __restrict_
     }
 }
 
+// The same product where tiles of 128 x 128 would leave most of the chip idle: few rows (down to a single token), or few of both.  A
+// workgroup takes 16 columns x 16 MT rows and its eight waves deal out the k-steps of 128 among them (v_mfma_scale_f32_16x16x128_f8f6f4);
+// operands go straight from memory to registers -- a lane's 16 bytes are one block -- and the waves' sums are joined in LDS in a fixed
+// order.  What bounds it is the latency of a handful of loads: 1 x 1280 -> 5120 takes MEASURED_1ROW.
+// SRC: the element type of x, quantised by the lane that feeds it to the instruction (a block's 32 values are one lane's; MT = 1 only, as
+// every column tile does it again), or uint8_t for codes.
+template <typename SRC, int MT, bool WIDE, typename T>
+__global__ __launch_bounds__(512) void k_mxfp4_linear_split(const SRC* __restrict__ x, const uint8_t* __restrict__ xs, int64_t ld,
+                                                            const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
+                                                            const float* __restrict__ bias, int M, int K, int N, int units, int act,
+                                                            T* __restrict__ y, int col_tiles) {
+    constexpr bool CODES = sizeof(SRC) == 1;
+    static_assert(CODES || MT == 1, "rows are quantised on the way for one row tile only");
+    __shared__ mx_f32x4 s_part[8][MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = lane & 15, q = lane >> 4;
+    const int n0 = (int)(blockIdx.x % (unsigned)col_tiles) * 16, m0 = (int)(blockIdx.x / (unsigned)col_tiles) * 16 * MT;
+    const int n = min(n0 + r, N - 1);
+    mx_f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+    // block 4 u + q of a row: byte (2 (u & 1) + q / 2) of the dword of (chunk u / 2, half q & 1)
+    auto scale = [&](const uint8_t* p, int rows, int row, int u) {
+        return (int)(reinterpret_cast<const uint32_t*>(p)[((size_t)(u >> 1) * 2 + (q & 1)) * rows + row] >> (16 * (u & 1) + 8 * (q >> 1)));
+    };
+#pragma unroll 2
+    for (int u = wave; u < units; u += 8) {
+        const int4 wq = *reinterpret_cast<const int4*>(w + (((size_t)u * 4 + q) * N + n) * 16);
+        const int sw = scale(ws, N, n, u);
+        const mx_i32x8 xw = {wq.x, wq.y, wq.z, wq.w, 0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            int4 xq = make_int4(0, 0, 0, 0);
+            int sx = 0;
+            if constexpr (CODES) {
+                const int m = min(m0 + 16 * t + r, M - 1);
+                xq = *reinterpret_cast<const int4*>(x + (((size_t)u * 4 + q) * M + m) * 16);
+                sx = scale(xs, M, m, u);
+            } else if (m0 + r < M) {
+                constexpr int V = MxVec<SRC>::N;
+                const int col = (u * 4 + q) * 32;
+                const SRC* src = x + (int64_t)(m0 + r) * ld + col;
+                float v[32];
+#pragma unroll
+                for (int g = 0; g < 32 / V; ++g) {
+                    if (WIDE && col + (g + 1) * V <= K) {
+                        const MxVec<SRC> c = *reinterpret_cast<const MxVec<SRC>*>(src + g * V);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) v[g * V + i] = (float)c.v[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) v[g * V + i] = col + g * V + i < K ? (float)src[g * V + i] : 0.f;
+                    }
+                }
+                uint32_t amax = 0;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+                sx = mx_scale_byte(amax);
+                const float sc = mx_scale_float(sx);
+                uint32_t d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t c = 0;
+                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i], v[8 * i + 1], sc, 0);
+                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 2], v[8 * i + 3], sc, 1);
+                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 4], v[8 * i + 5], sc, 2);
+                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 6], v[8 * i + 7], sc, 3);
+                    d[i] = sx == 255 ? 0x77777777u : c;
+                }
+                xq = make_int4((int)d[0], (int)d[1], (int)d[2], (int)d[3]);
+            }
+            const mx_i32x8 xx = {xq.x, xq.y, xq.z, xq.w, 0, 0, 0, 0};
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(xw, xx, acc[t], 4, 4, 0, sw, 0, sx);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) s_part[wave][t][lane] = acc[t];
+    __syncthreads();
+    // element (lane, e): row lane & 15, column 4 (lane >> 4) + e
+    for (int i = threadIdx.x; i < MT * 256; i += 512) {
+        const int col = i & 15, row = i >> 4;  // consecutive threads: consecutive columns
+        const int m = m0 + row, nn = n0 + col;
+        if (m >= M || nn >= N) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) sum += s_part[p][row >> 4][(col >> 2) * 16 + (row & 15)][col & 3];
+        y[(int64_t)m * N + nn] = (T)mx_act(sum + (bias ? bias[nn] : 0.f), act);
+    }
+}
+
 static bool mx_aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 template <typename T>
@@ -306,16 +396,54 @@ static int mx_dequantize_t(const uint8_t* codes, const uint8_t* scales, int M, i
     return SNF_OK;
 }
 
+// Tiles of 128 x 128 fill the chip from about 128 of them; below that the split kernel's 16 x 64 (or 16 x 16) do better:
+// MEASURED_SPLIT
+static bool mx_split(int M, int N) { return (int64_t)ceil_div(M, 128) * ceil_div(N, 128) < 128; }
+
 template <typename T>
 static int mx_linear_t(const uint8_t* a, const uint8_t* as, const uint8_t* w, const uint8_t* ws, const float* bias, int M, int K, int N,
                        int act, T* y, hipStream_t st) {
     constexpr int BM = 128, BN = 128;
-    const int chunks = ceil_div(K, 256), rts = ceil_div(M, BM), cts = ceil_div(N, BN);
+    const int chunks = ceil_div(K, 256);
+    if (mx_split(M, N)) {
+        const int cts = ceil_div(N, 16), mt = M <= 16 ? 1 : M <= 32 ? 2 : 4, rts = ceil_div(M, 16 * mt);
+        SNF_REQUIRE((int64_t)rts * cts * 512 < ((int64_t)1 << 32), "snf_mxfp4_linear: %d x %d is too large for one launch", M, N);
+        const dim3 grid((unsigned)(rts * cts)), block(512);
+        if (mt == 1) k_mxfp4_linear_split<uint8_t, 1, true, T><<<grid, block, 0, st>>>(a, as, 0, w, ws, bias, M, K, N, 2 * chunks, act, y, cts);
+        else if (mt == 2) k_mxfp4_linear_split<uint8_t, 2, true, T><<<grid, block, 0, st>>>(a, as, 0, w, ws, bias, M, K, N, 2 * chunks, act, y, cts);
+        else k_mxfp4_linear_split<uint8_t, 4, true, T><<<grid, block, 0, st>>>(a, as, 0, w, ws, bias, M, K, N, 2 * chunks, act, y, cts);
+        SNF_LAUNCH_CHECK("snf_mxfp4_linear (split)");
+        return SNF_OK;
+    }
+    const int rts = ceil_div(M, BM), cts = ceil_div(N, BN);
     SNF_REQUIRE(((int64_t)rts * cts + 8) * 256 < ((int64_t)1 << 32), "snf_mxfp4_linear: %d x %d is too large for one launch", M, N);
     const int per = (rts * cts + 7) / 8;
     k_mxfp4_linear<BM, BN, T><<<dim3(8 * per), dim3(256), 2 * 8 * (BM + BN) * 16, st>>>(a, as, w, ws, bias, M, N, chunks, act, y, rts, cts);
     SNF_LAUNCH_CHECK("snf_mxfp4_linear");
     return SNF_OK;
+}
+
+template <typename SRC, typename T>
+static int mx_rows_t(const SRC* x, int64_t ld, const uint8_t* w, const uint8_t* ws, const float* bias, int M, int K, int N, int act, T* y,
+                     hipStream_t st) {
+    const int cts = ceil_div(N, 16), units = 2 * ceil_div(K, 256);
+    if (mx_aligned(x, 16) && (ld * (int64_t)sizeof(SRC)) % 16 == 0)
+        k_mxfp4_linear_split<SRC, 1, true, T><<<dim3(cts), dim3(512), 0, st>>>(x, nullptr, ld, w, ws, bias, M, K, N, units, act, y, cts);
+    else
+        k_mxfp4_linear_split<SRC, 1, false, T><<<dim3(cts), dim3(512), 0, st>>>(x, nullptr, ld, w, ws, bias, M, K, N, units, act, y, cts);
+    SNF_LAUNCH_CHECK("snf_mxfp4_linear_rows");
+    return SNF_OK;
+}
+
+template <typename SRC>
+static int mx_rows_src(const SRC* x, int64_t ld, const uint8_t* w, const uint8_t* ws, const float* bias, int M, int K, int N, int act,
+                       void* y, int out_dtype, hipStream_t st) {
+    switch (out_dtype) {
+        case SNF_F32: return mx_rows_t(x, ld, w, ws, bias, M, K, N, act, (float*)y, st);
+        case SNF_BF16: return mx_rows_t(x, ld, w, ws, bias, M, K, N, act, (__bf16*)y, st);
+        case SNF_F16: return mx_rows_t(x, ld, w, ws, bias, M, K, N, act, (_Float16*)y, st);
+    }
+    SNF_REQUIRE(false, "snf_mxfp4_linear_rows: unknown dtype %d", out_dtype);
 }
 
 }  // namespace snf
@@ -367,6 +495,23 @@ int snf_mxfp4_linear(const uint8_t* a_codes, const uint8_t* a_scales, const uint
         case SNF_F16: return snf::mx_linear_t(a_codes, a_scales, w_codes, w_scales, bias, M, K, N, act, (_Float16*)y, st);
     }
     SNF_REQUIRE(false, "snf_mxfp4_linear: unknown dtype %d", dtype);
+}
+
+int snf_mxfp4_linear_rows(const void* x, int dtype, int64_t ld, const uint8_t* w_codes, const uint8_t* w_scales, const float* bias, int M,
+                          int K, int N, int act, void* y, int out_dtype, snf_stream_t stream) {
+    SNF_REQUIRE(M >= 0 && M <= SNF_MXFP4_ROWS && K >= 1 && N >= 1, "snf_mxfp4_linear_rows: bad sizes M=%d K=%d N=%d", M, K, N);
+    SNF_REQUIRE(act >= SNF_ACT_NONE && act <= SNF_ACT_GELU, "snf_mxfp4_linear_rows: unknown activation %d", act);
+    if (M == 0) return SNF_OK;
+    SNF_REQUIRE(x && w_codes && w_scales && y, "snf_mxfp4_linear_rows: null pointer");
+    SNF_REQUIRE(ld >= K || M == 1, "snf_mxfp4_linear_rows: rows of %d values overlap at stride %lld", K, (long long)ld);
+    SNF_REQUIRE(snf::mx_aligned(w_codes, 16) && snf::mx_aligned(w_scales, 4), "snf_mxfp4_linear_rows: an operand is not aligned");
+    hipStream_t st = (hipStream_t)stream;
+    switch (dtype) {
+        case SNF_F32: return snf::mx_rows_src((const float*)x, ld, w_codes, w_scales, bias, M, K, N, act, y, out_dtype, st);
+        case SNF_BF16: return snf::mx_rows_src((const __bf16*)x, ld, w_codes, w_scales, bias, M, K, N, act, y, out_dtype, st);
+        case SNF_F16: return snf::mx_rows_src((const _Float16*)x, ld, w_codes, w_scales, bias, M, K, N, act, y, out_dtype, st);
+    }
+    SNF_REQUIRE(false, "snf_mxfp4_linear_rows: unknown dtype %d", dtype);
 }
 
 }  // extern "C"

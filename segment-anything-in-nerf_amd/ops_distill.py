@@ -43,7 +43,6 @@ def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty((nbytes // 8,), device=device, dtype=torch.int64) if nbytes else None
 
 
-@torch.no_grad()
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     """The k largest of logits [..., V] with their places and the log-sum-exp of logits / temperature over all other places.  Equal logits
     come in the order of their places; a NaN counts as larger than everything.  k <= min(V, 256)."""
@@ -59,7 +58,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     rest = torch.empty(lead, device=dev, dtype=torch.float32)
     R = rest.numel()
     if R:
-        x, ld = _rows(logits.unsqueeze(0) if logits.dim() == 1 else logits)
+        x, ld = _rows((logits.unsqueeze(0) if logits.dim() == 1 else logits).detach())
         code = DTYPE_CODE[x.dtype]
         nbytes = int(_L().snf_top_logits_workspace_bytes(R, V, k, code))
         ws = _workspace(nbytes, dev)
@@ -68,53 +67,57 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     return TopLogits(ids, vals, rest)
 
 
-def _saved_parts(saved: torch.Tensor, R: int):
-    return saved[:4 * R], saved[4 * R:5 * R], saved[5 * R:]
-
-
 class _TopDistill(torch.autograd.Function):
+    # one buffer of floats: stats [R, 4], p [R, K], counted [R], the divisor, rows [R] (unless they are the result)
     @staticmethod
     def forward(ctx, student, ids, logits, rest, temperature: float, weight: float, reduction: str):
         dev = student.device
         V, K = int(student.shape[-1]), int(ids.shape[-1])
-        lead = tuple(student.shape[:-1])
         z, ld = _rows(student.unsqueeze(0) if student.dim() == 1 else student)
         ids, logits = ids.contiguous(), logits.contiguous()
         rest = rest.contiguous() if rest is not None else None
         R = z.shape[0]
-        code, st = DTYPE_CODE[z.dtype], _stream_on(dev)
-        rows = torch.empty(lead, device=dev, dtype=torch.float32)
-        saved = torch.empty((R * (5 + K),), device=dev, dtype=torch.float32)  # stats [R, 4], counted [R], p [R, K]
-        stats, counted, p = _saved_parts(saved, R)
-        if R:
+        code = DTYPE_CODE[z.dtype]
+        per_row = reduction == "none"
+        saved = torch.empty((R * (6 + K) + 1,), device=dev, dtype=torch.float32)
+        at = saved.data_ptr()
+        counted, divisor, rows = at + 4 * R * (4 + K), at + 4 * R * (5 + K), at + 4 * R * (5 + K) + 4
+        loss = torch.empty(tuple(student.shape[:-1]) if per_row else (), device=dev, dtype=torch.float32)
+        if R or not per_row:
             nbytes = int(_L().snf_top_distill_workspace_bytes(R, V, code))
             ws = _workspace(nbytes, dev)
             _launch("snf_top_distill_fwd", _p(z), code, R, V, ld, _p(ids), int(ids.dtype == torch.int64), _p(logits),
-                    DTYPE_CODE[logits.dtype], _p(rest), K, temperature, weight, _p(rows), _p(counted), _p(stats), _p(p), _p(ws), nbytes, st,
+                    DTYPE_CODE[logits.dtype], _p(rest), K, temperature, weight, _p(loss) if per_row else rows, counted, at, at + 16 * R,
+                    int(reduction == "mean"), None if per_row else _p(loss), divisor, _p(ws), nbytes, _stream_on(dev),
                     units=float(R * V * z.element_size()))
-        loss, divisor = rows, None
-        if reduction != "none":
-            loss, divisor = (torch.empty((), device=dev, dtype=torch.float32) for _ in range(2))
-            _launch("snf_top_distill_mean", _p(rows), _p(counted), R, int(reduction == "mean"), _p(loss), _p(divisor), st)
-        ctx.args = (tuple(student.shape), R, V, ld, K, temperature, weight, reduction)
-        ctx.save_for_backward(z, ids, saved, divisor)
+        ctx.args = (student.shape, R, V, ld, K, temperature, weight, per_row)
+        ctx.save_for_backward(z, ids, saved)
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        z, ids, saved, divisor = ctx.saved_tensors
-        shape, R, V, ld, K, temperature, weight, reduction = ctx.args
+        if torch.is_grad_enabled():  # create_graph: a second derivative is refused when it is asked for
+            return _TopDistill._refusing_twice(ctx, g)
+        return _TopDistill._gradient(ctx, g)
+
+    @staticmethod
+    def _gradient(ctx, g):
         if not ctx.needs_input_grad[0]:
             return (None,) * 7
+        z, ids, saved = ctx.saved_tensors
+        shape, R, V, ld, K, temperature, weight, per_row = ctx.args
         dz = torch.empty(shape, device=z.device, dtype=z.dtype)
         if R:
-            g = g.to(torch.float32).contiguous()
-            stats, counted, p = _saved_parts(saved, R)
+            if g.dtype != torch.float32 or not g.is_contiguous():
+                g = g.to(torch.float32).contiguous()
+            at = saved.data_ptr()
+            counted, divisor = at + 4 * R * (4 + K), at + 4 * R * (5 + K)
             _launch("snf_top_distill_bwd", _p(z), DTYPE_CODE[z.dtype], R, V, ld, _p(ids), int(ids.dtype == torch.int64), K, temperature,
-                    weight, _p(g), int(reduction == "none"), _p(divisor), _p(counted), _p(stats), _p(p), _p(dz), _stream_on(z.device),
+                    weight, _p(g), int(per_row), None if per_row else divisor, counted, at, at + 16 * R, _p(dz), _stream_on(z.device),
                     units=float(2 * R * V * z.element_size()))
         return dz, None, None, None, None, None, None
+
+    _refusing_twice = staticmethod(once_differentiable(_gradient.__func__))
 
 
 def top_logits_distill_loss(student: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor, rest: Optional[torch.Tensor] = None,

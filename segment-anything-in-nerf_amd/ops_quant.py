@@ -11,6 +11,7 @@ from ._opcore import ACT_GELU, ACT_NONE, DTYPE_CODE, _dev, _launch, _p, _rows, _
 __all__ = ["MXFP4_BLOCK", "Mxfp4", "quantize_mxfp4", "dequantize_mxfp4", "linear_mxfp4"]
 
 MXFP4_BLOCK = 32  # values that share a scale
+MXFP4_ROWS = 16   # SNF_MXFP4_ROWS
 
 
 class Mxfp4:
@@ -39,6 +40,13 @@ class Mxfp4:
             raise ValueError(f"Mxfp4: {self.shape} is not a shape of {self.M} rows of {self.K}")
         self.codes, self.scales = codes, scales
 
+    @classmethod
+    def _of(cls, codes, scales, K: int, shape) -> "Mxfp4":
+        """What quantize_mxfp4 has just laid out: nothing left to check."""
+        q = object.__new__(cls)
+        q.codes, q.scales, q.M, q.K, q.shape = codes, scales, codes.shape[1], K, shape
+        return q
+
     @property
     def device(self) -> torch.device:
         return self.codes.device
@@ -48,7 +56,6 @@ class Mxfp4:
         return dequantize_mxfp4(self)
 
 
-@torch.no_grad()
 def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
     """x [..., K] (float32 / bfloat16 / float16; rows may be strided) -> Mxfp4.  Per block of 32 along K the scale is
     2^max(floor(log2 max|x|) - 2, -127); values are rounded to the nearest code (halves to even), magnitudes above 6 scales become 6.
@@ -66,13 +73,12 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
     codes = torch.empty((8 * chunks, M, 16), device=dev, dtype=torch.uint8)
     scales = torch.empty((2 * chunks, M, 4), device=dev, dtype=torch.uint8)
     if M:
-        x, ld = _rows(x)
+        x, ld = _rows(x.detach())
         _launch("snf_mxfp4_quantize", _p(x), DTYPE_CODE[x.dtype], M, K, ld, _p(codes), _p(scales), _stream_on(dev),
                 units=float(M * K * x.element_size()))
-    return Mxfp4(codes, scales, K, shape)
+    return Mxfp4._of(codes, scales, K, shape)
 
 
-@torch.no_grad()
 def dequantize_mxfp4(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that `q` holds, in its shape.  float32 holds every value exactly; so does the type that was quantised."""
     if not isinstance(q, Mxfp4):
@@ -87,7 +93,6 @@ def dequantize_mxfp4(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tens
     return out
 
 
-@torch.no_grad()
 def linear_mxfp4(x: Union[torch.Tensor, Mxfp4], w: Mxfp4, bias: Optional[torch.Tensor] = None, act: int = ACT_NONE,
                  out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """act(x W^T + bias) with both operands in 4 bits and float32 sums: x [..., K] is quantised on the way in (or comes as an Mxfp4),
@@ -118,7 +123,15 @@ def linear_mxfp4(x: Union[torch.Tensor, Mxfp4], w: Mxfp4, bias: Optional[torch.T
     y = torch.empty(tuple(x.shape[:-1]) + (w.M,), device=dev, dtype=out_dtype)
     if y.numel() == 0:
         return y
-    q = x if isinstance(x, Mxfp4) else quantize_mxfp4(x)
+    if isinstance(x, Mxfp4):
+        q = x
+    elif y.numel() <= MXFP4_ROWS * w.M:  # few rows: quantised on the way into the product, one launch
+        x, ld = _rows((x.unsqueeze(0) if x.dim() == 1 else x).detach())
+        _launch("snf_mxfp4_linear_rows", _p(x), DTYPE_CODE[x.dtype], ld, _p(w.codes), _p(w.scales), _p(bias), x.shape[0], w.K, w.M, int(act),
+                _p(y), DTYPE_CODE[out_dtype], _stream_on(dev), tag=f"{w.K}x{w.M}", units=2.0 * y.numel() * w.K)
+        return y
+    else:
+        q = quantize_mxfp4(x)
     _launch("snf_mxfp4_linear", _p(q.codes), _p(q.scales), _p(w.codes), _p(w.scales), _p(bias), q.M, q.K, w.M, int(act), _p(y),
             DTYPE_CODE[out_dtype], _stream_on(dev), tag=f"{q.K}x{w.M}", units=2.0 * q.M * q.K * w.M)
     return y

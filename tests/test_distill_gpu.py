@@ -347,7 +347,7 @@ def test_distill_leaves_teacher_and_neighbours_alone():
     dz = torch.full((R * V + 64,), 7.0, device="cuda", dtype=torch.bfloat16)
     st = C._stream()
     C._launch("snf_top_distill_fwd", C._p(z), 1, R, V, V, C._p(ids), 0, C._p(top), 1, C._p(rest), K, 1.0, 1.0, C._p(rows), C._p(cnt),
-              C._p(stats), C._p(p), None, 0, st)
+              C._p(stats), C._p(p), 0, None, None, None, 0, st)
     one = torch.ones(1, **f32)
     for off in (0, 1):  # rows of the gradient at the student's offsets from 16 bytes, and at others
         dz.fill_(7.0)
@@ -413,10 +413,10 @@ def test_refusals_at_the_library():
         C._launch("snf_top_logits", C._p(x), 0, 1, 200000, 200000, 3, 1.0, C._p(i), C._p(x), C._p(x), None, 0, C._stream())
     with pytest.raises(_lib.SnfError, match="workspace"):
         C._launch("snf_top_distill_fwd", C._p(x), 0, 1, 200000, 200000, C._p(i), 0, C._p(x), 0, None, 3, 1.0, 1.0, C._p(x), C._p(x), C._p(x),
-                  C._p(x), None, 0, C._stream())
+                  C._p(x), 0, None, None, None, 0, C._stream())
     with pytest.raises(_lib.SnfError):
         C._launch("snf_top_distill_fwd", C._p(x), 0, 4, 64, 64, C._p(i), 0, C._p(x), 0, None, 257, 1.0, 1.0, C._p(x), C._p(x), C._p(x), C._p(x),
-                  None, 0, C._stream())
+                  0, None, None, None, 0, C._stream())
     with pytest.raises(_lib.SnfError):
         C._launch("snf_top_distill_bwd", C._p(x), 0, 4, 64, 64, C._p(i), 0, 3, 1.0, 1.0, None, 0, None, C._p(x), C._p(x), C._p(x), C._p(x),
                   C._stream())
