@@ -11,6 +11,7 @@
 //                                  1 KB that one global -> LDS copy of a wave moves, in the order in which the fragments are read
 //     scales [Kp / 256][2][M][4]   byte j of (chunk, half, row): block 8 chunk + 2 j + half.  One dword holds a lane's scales of the four
 //                                  k-steps of a 256 chunk; the instruction picks the byte.
+#include <type_traits>
 #include "common.hpp"
 
 namespace snf {
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(256) void k_mxfp4_dequantize(const uint8_t* __restr
         }
         T* dst = out + (int64_t)row * K + col;
         if (WIDE && col + V <= K) {
-            *reinterpret_cast<MxVec<T>*>(dst) = o;
+            __builtin_nontemporal_store(__builtin_bit_cast(mx_f32x4, o), reinterpret_cast<mx_f32x4*>(dst));  // (84 MB: 17.2 us; through the caches 20.2)
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
@@ -154,35 +155,57 @@ __global__ __launch_bounds__(256) void k_mxfp4_dequantize(const uint8_t* __restr
 }
 
 // ---- product --------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float mx_act(float v, int act) {
+template <int ACT>
+__device__ __forceinline__ float mx_act(float v) {
+    if constexpr (ACT == SNF_ACT_RELU) return v > 0.f || v != v ? v : 0.f;
+    else if constexpr (ACT == SNF_ACT_SIGMOID) return 1.f / (1.f + expf(-v));
+    else if constexpr (ACT == SNF_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    else return v;
+}
+// f with the activation as a constant: one copy of an epilogue each, no branch per element
+template <typename F>
+__device__ __forceinline__ void mx_with_act(int act, F f) {
     switch (act) {
-        case SNF_ACT_RELU: return v > 0.f || v != v ? v : 0.f;
-        case SNF_ACT_SIGMOID: return 1.f / (1.f + expf(-v));
-        case SNF_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-        default: return v;
+        case SNF_ACT_RELU: f(std::integral_constant<int, SNF_ACT_RELU>{}); break;
+        case SNF_ACT_SIGMOID: f(std::integral_constant<int, SNF_ACT_SIGMOID>{}); break;
+        case SNF_ACT_GELU: f(std::integral_constant<int, SNF_ACT_GELU>{}); break;
+        default: f(std::integral_constant<int, SNF_ACT_NONE>{});
     }
 }
 
+constexpr int MX_PITCH = 64 + 4;  // floats of a row of the outgoing tile in LDS
+constexpr int mx_stage(int bm, int bn) { return (8 * 16 + 2 * 4) * (bm + bn); }
+
 // y[m][n] = act(sum_k a[m][k] w[n][k] + bias[n]), fp32 sums on v_mfma_scale_f32_32x32x64_f8f6f4 (products of codes are exact).
-// A workgroup of four waves (2 x 2) takes BM rows x BN columns, a wave (BM / 2) x (BN / 2); a stage is 256 k of both operands in LDS, two
-// stage buffers: the copies of the next stage run under the products of this one.  The weights are the instruction's first operand, so a
-// lane ends up with four consecutive columns of one row.
-template <int BM, int BN, typename T>
-__global__ __launch_bounds__(256) void k_mxfp4_linear(const uint8_t* __restrict__ a, const uint8_t* __restrict__ as,
-                                                      const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
-                                                      const float* __restrict__ bias, int M, int N, int chunks, int act,
-                                                      T* __restrict__ y, int row_tiles, int col_tiles) {
-    constexpr int RB = BM / 64, CB = BN / 64;  // 32-row / 32-column blocks of a wave
-    constexpr int A_BYTES = 8 * BM * 16, W_BYTES = 8 * BN * 16, STAGE = A_BYTES + W_BYTES;
+// A workgroup of WM x WN waves takes BM rows x BN columns; a stage is 256 k of both operands and their scales in LDS, two stage buffers:
+// the copies of the next stage are under way during the products of this one.  The weights are the instruction's first operand: a lane
+// ends up with four consecutive columns of one row, and the tile leaves through LDS in whole rows of 64 columns, where the bias and the
+// activation are applied; its stores do not stay in the caches (they are half of a wide layer's time: 4900 x 1280 -> 3840 fp32 36 us with
+// ordinary stores, 32 with these).
+// Measured: 4900 x 1280 -> 3840 fp32 (75 MB out) 28 us = 1.7 PFLOP/s, 2.7 TB/s of stores; 16384 x 5120 -> 5120 fp32 243 us = 3.5 PFLOP/s.
+template <int BM, int BN, int WM, int WN, typename T>
+__global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_linear(const uint8_t* __restrict__ a, const uint8_t* __restrict__ as,
+                                                               const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
+                                                               const float* __restrict__ bias, int M, int N, int chunks, int act,
+                                                               T* __restrict__ y, int row_tiles, int col_tiles) {
+    constexpr int WAVES = WM * WN, RB = BM / WM / 32, CB = BN / WN / 32;  // 32-row / 32-column blocks of a wave
+    // a stage: codes of the rows [8][BM][16], of the columns [8][BN][16], scales of the rows [2][BM][4], of the columns [2][BN][4]
+    constexpr int W_AT = 8 * BM * 16, SA_AT = W_AT + 8 * BN * 16, SW_AT = SA_AT + 8 * BM, STAGE = mx_stage(BM, BN);
+    constexpr int A_PIECES = BM / 8 / WAVES, W_PIECES = BN / 8 / WAVES;  // 1 KB copies of a wave a stage: 64 rows of one block
+    constexpr int S_PIECES = (BM + BN) / 32 / WAVES;                     // 256-byte copies: 64 rows' scales of one half
+    constexpr int PITCH = MX_PITCH;
+    static_assert(CB % 2 == 0 && A_PIECES * WAVES * 8 == BM && W_PIECES * WAVES * 8 == BN && S_PIECES * WAVES * 32 == BM + BN, "tile");
     extern __shared__ __attribute__((aligned(16))) uint8_t mx_lds[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int li = lane & 31, half = lane >> 5, wr = wave >> 1, wc = wave & 1;
-    // consecutive tiles of one XCD share their rows' operand in its L2
+    const int li = lane & 31, half = lane >> 5, wr = wave / WN, wc = wave % WN;
+    // an XCD takes consecutive tiles, and those go down 8 row tiles before they step to the next column tile: the workgroups that run
+    // together on it work on an 8 x 8 square of tiles, whose operands its L2 holds
     const int total = row_tiles * col_tiles, per = (total + 7) >> 3;
     const int slot = (int)blockIdx.x >> 3, t = ((int)blockIdx.x & 7) * per + slot;
     if (slot >= per || t >= total) return;
-    const int rt = t / col_tiles, ct = t - rt * col_tiles;
+    const int group = t / (8 * col_tiles), in_group = t - group * 8 * col_tiles, tall = min(8, row_tiles - group * 8);
+    const int rt = group * 8 + in_group % tall, ct = in_group / tall;
     const int m0 = rt * BM, n0 = ct * BN;
 
     mx_f32x16 acc[RB][CB];
@@ -193,43 +216,42 @@ __global__ __launch_bounds__(256) void k_mxfp4_linear(const uint8_t* __restrict_
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-    // rows past the end read the last row (their results are not stored)
-    auto copy = [&](int c, int buf) {
-        uint8_t* dst = mx_lds + buf * STAGE;
+    // rows past the end read the last row (their results are not stored).  A wave copies the same 64 rows of every block it has: one
+    // 32-bit offset a lane (M, N < 2^28) on top of addresses that are the wave's
+    static_assert(WAVES % (BM / 64) == 0 && WAVES % (BN / 64) == 0, "a wave's rows");
+    const uint32_t off_a = (uint32_t)min(m0 + wave % (BM / 64) * 64 + lane, M - 1) * 16u;
+    const uint32_t off_w = (uint32_t)min(n0 + wave % (BN / 64) * 64 + lane, N - 1) * 16u;
+    auto copy = [&](int c, uint8_t* __restrict__ stage) {
+        uint8_t* dst = stage + wave * 1024;
 #pragma unroll
-        for (int p = 0; p < 8 * (BM / 64) / 4; ++p) {
-            const int piece = p * 4 + wave, kb = piece / (BM / 64), g = piece % (BM / 64);
-            const int row = min(m0 + g * 64 + lane, M - 1);
-            __builtin_amdgcn_global_load_lds((mx_gptr)(a + (((size_t)c * 8 + kb) * M + row) * 16), (mx_lptr)(dst + (kb * BM + g * 64) * 16), 16,
-                                             0, 0);
+        for (int p = 0; p < A_PIECES; ++p) {
+            const uint8_t* block = a + ((size_t)c * 8 + (p * WAVES + wave) / (BM / 64)) * M * 16;
+            __builtin_amdgcn_global_load_lds((mx_gptr)(block + off_a), (mx_lptr)(dst + p * WAVES * 1024), 16, 0, 0);
         }
 #pragma unroll
-        for (int p = 0; p < 8 * (BN / 64) / 4; ++p) {
-            const int piece = p * 4 + wave, kb = piece / (BN / 64), g = piece % (BN / 64);
-            const int row = min(n0 + g * 64 + lane, N - 1);
-            __builtin_amdgcn_global_load_lds((mx_gptr)(w + (((size_t)c * 8 + kb) * N + row) * 16),
-                                             (mx_lptr)(dst + A_BYTES + (kb * BN + g * 64) * 16), 16, 0, 0);
+        for (int p = 0; p < W_PIECES; ++p) {
+            const uint8_t* block = w + ((size_t)c * 8 + (p * WAVES + wave) / (BN / 64)) * N * 16;
+            __builtin_amdgcn_global_load_lds((mx_gptr)(block + off_w), (mx_lptr)(dst + W_AT + p * WAVES * 1024), 16, 0, 0);
+        }
+#pragma unroll
+        for (int p = 0; p < S_PIECES; ++p) {
+            const int piece = p * WAVES + wave;  // rows' first
+            const bool rows = piece < BM / 32;
+            const int at = rows ? piece : piece - BM / 32, h = at / ((rows ? BM : BN) / 64), g = at % ((rows ? BM : BN) / 64);
+            const int count = rows ? M : N;
+            const uint8_t* half_ = (rows ? as : ws) + ((size_t)c * 2 + h) * count * 4;
+            __builtin_amdgcn_global_load_lds((mx_gptr)(half_ + (uint32_t)min((rows ? m0 : n0) + g * 64 + lane, count - 1) * 4u),
+                                             (mx_lptr)(stage + SA_AT + piece * 256), 4, 0, 0);
         }
     };
-    int arow[RB], wrow[CB];
-#pragma unroll
-    for (int i = 0; i < RB; ++i) arow[i] = min(m0 + wr * (BM / 2) + i * 32 + li, M - 1);
-#pragma unroll
-    for (int j = 0; j < CB; ++j) wrow[j] = min(n0 + wc * (BN / 2) + j * 32 + li, N - 1);
-    const int* as32 = reinterpret_cast<const int*>(as);
-    const int* ws32 = reinterpret_cast<const int*>(ws);
-
-    copy(0, 0);
-    __syncthreads();
-    for (int c = 0; c < chunks; ++c) {
-        if (c + 1 < chunks) copy(c + 1, (c + 1) & 1);
+    auto multiply = [&](const uint8_t* __restrict__ st) {
+        const uint8_t* fa = st + (half * BM + wr * RB * 32 + li) * 16;
+        const uint8_t* fw = st + W_AT + (half * BN + wc * CB * 32 + li) * 16;
         int sa[RB], sw[CB];
 #pragma unroll
-        for (int i = 0; i < RB; ++i) sa[i] = as32[((size_t)c * 2 + half) * M + arow[i]];
+        for (int i = 0; i < RB; ++i) sa[i] = *reinterpret_cast<const int*>(st + SA_AT + (half * BM + (wr * RB + i) * 32 + li) * 4);
 #pragma unroll
-        for (int j = 0; j < CB; ++j) sw[j] = ws32[((size_t)c * 2 + half) * N + wrow[j]];
-        const uint8_t* fa = mx_lds + (c & 1) * STAGE + (half * BM + wr * (BM / 2) + li) * 16;
-        const uint8_t* fw = mx_lds + (c & 1) * STAGE + A_BYTES + (half * BN + wc * (BN / 2) + li) * 16;
+        for (int j = 0; j < CB; ++j) sw[j] = *reinterpret_cast<const int*>(st + SW_AT + (half * BN + (wc * CB + j) * 32 + li) * 4);
         // the scale's byte is part of the instruction
 #define MX_STEP(S_)                                                                                                              \
     {                                                                                                                            \
@@ -250,38 +272,72 @@ __global__ __launch_bounds__(256) void k_mxfp4_linear(const uint8_t* __restrict_
         MX_STEP(2)
         MX_STEP(3)
 #undef MX_STEP
+    };
+    // (the pointers are restricted so that the reads of one buffer are known not to wait for the copies into the other)
+    auto step = [&](const uint8_t* __restrict__ from, uint8_t* __restrict__ into, int c) {
+        copy(c + 1, into);
+        multiply(from);
+        __builtin_amdgcn_sched_barrier(0);  // (the wait for the copies belongs behind the products)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-    }
-    // element e of a lane: column 8 (e / 4) + 4 half + e % 4 of the block, row li
-    const bool wide = N % 4 == 0;
+    };
+    uint8_t *const even = mx_lds, *const odd = mx_lds + STAGE;
+    copy(0, even);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int c = 0; c + 1 < chunks; ++c) step(c & 1 ? odd : even, c & 1 ? even : odd, c);
+    multiply((chunks - 1) & 1 ? odd : even);
+    __syncthreads();
+    // out, 32 rows x 64 columns at a time through the wave's own piece of LDS.  Element e of a lane: column 8 (e / 4) + 4 half + e % 4 of
+    // its 32-column block, row li.
+    float* out = reinterpret_cast<float*>(mx_lds) + wave * 32 * PITCH;
+    constexpr int V = MxVec<T>::N, LPR = 64 / V, RPP = 64 / LPR;  // columns a lane stores at once; lanes of a row; rows of a pass
+    const bool wide = N % V == 0;
+    mx_with_act(act, [&](auto fixed) {
 #pragma unroll
-    for (int i = 0; i < RB; ++i) {
-        const int m = m0 + wr * (BM / 2) + i * 32 + li;
-        if (m >= M) continue;
+        for (int j2 = 0; j2 < CB / 2; ++j2) {
+            const int nb = n0 + (wc * CB + 2 * j2) * 32, col = (lane % LPR) * V;
+            float b[V];
 #pragma unroll
-        for (int j = 0; j < CB; ++j)
+            for (int e = 0; e < V; ++e) b[e] = bias && nb + col + e < N ? bias[nb + col + e] : 0.f;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int n = n0 + wc * (BN / 2) + j * 32 + 8 * g + 4 * half;
-                struct alignas(4 * sizeof(T)) { T v[4]; } o;
+            for (int i = 0; i < RB; ++i) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o.v[e] = (T)mx_act(acc[i][j][4 * g + e] + (bias && n + e < N ? bias[n + e] : 0.f), act);
-                T* dst = y + (int64_t)m * N + n;
-                if (wide) {
-                    if (n < N) *reinterpret_cast<decltype(o)*>(dst) = o;
-                } else {
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (n + e < N) dst[e] = o.v[e];
+                    for (int g = 0; g < 4; ++g) {
+                        const mx_f32x16& v = acc[i][2 * j2 + j];
+                        *reinterpret_cast<mx_f32x4*>(out + li * PITCH + 32 * j + 8 * g + 4 * half) =
+                            mx_f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+                    }
+                __builtin_amdgcn_wave_barrier();
+                const int mb = m0 + (wr * RB + i) * 32;
+#pragma unroll
+                for (int p = 0; p < 32 / RPP; ++p) {
+                    const int row = p * RPP + lane / LPR;
+                    MxVec<T> o;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) o.v[e] = (T)mx_act<decltype(fixed)::value>(out[row * PITCH + col + e] + b[e]);
+                    if (mb + row >= M || nb + col >= N) continue;
+                    T* dst = y + (int64_t)(mb + row) * N + nb + col;
+                    if (wide) {
+                        __builtin_nontemporal_store(__builtin_bit_cast(mx_f32x4, o), reinterpret_cast<mx_f32x4*>(dst));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; ++e)
+                            if (nb + col + e < N) dst[e] = o.v[e];
+                    }
                 }
+                __builtin_amdgcn_wave_barrier();
             }
-    }
+        }
+    });
 }
 
 // The same product where tiles of 128 x 128 would leave most of the chip idle: few rows (down to a single token), or few of both.  A
 // workgroup takes 16 columns x 16 MT rows and its eight waves deal out the k-steps of 128 among them (v_mfma_scale_f32_16x16x128_f8f6f4);
 // operands go straight from memory to registers -- a lane's 16 bytes are one block -- and the waves' sums are joined in LDS in a fixed
-// order.  What bounds it is the latency of a handful of loads: 1 x 1280 -> 5120 takes MEASURED_1ROW.
+// order.  What bounds it is the latency of a few loads one behind the other: 1 x 1280 -> 5120 takes 5.0 us (3.5 MB of weights: 0.5 us).
 // SRC: the element type of x, quantised by the lane that feeds it to the instruction (a block's 32 values are one lane's; MT = 1 only, as
 // every column tile does it again), or uint8_t for codes.
 template <typename SRC, int MT, bool WIDE, typename T>
@@ -357,15 +413,17 @@ __global__ __launch_bounds__(512) void k_mxfp4_linear_split(const SRC* __restric
     for (int t = 0; t < MT; ++t) s_part[wave][t][lane] = acc[t];
     __syncthreads();
     // element (lane, e): row lane & 15, column 4 (lane >> 4) + e
-    for (int i = threadIdx.x; i < MT * 256; i += 512) {
-        const int col = i & 15, row = i >> 4;  // consecutive threads: consecutive columns
-        const int m = m0 + row, nn = n0 + col;
-        if (m >= M || nn >= N) continue;
-        float sum = 0.f;
+    mx_with_act(act, [&](auto fixed) {
+        for (int i = threadIdx.x; i < MT * 256; i += 512) {
+            const int col = i & 15, row = i >> 4;  // consecutive threads: consecutive columns
+            const int m = m0 + row, nn = n0 + col;
+            if (m >= M || nn >= N) continue;
+            float sum = 0.f;
 #pragma unroll
-        for (int p = 0; p < 8; ++p) sum += s_part[p][row >> 4][(col >> 2) * 16 + (row & 15)][col & 3];
-        y[(int64_t)m * N + nn] = (T)mx_act(sum + (bias ? bias[nn] : 0.f), act);
-    }
+            for (int p = 0; p < 8; ++p) sum += s_part[p][row >> 4][(col >> 2) * 16 + (row & 15)][col & 3];
+            y[(int64_t)m * N + nn] = (T)mx_act<decltype(fixed)::value>(sum + (bias ? bias[nn] : 0.f));
+        }
+    });
 }
 
 static bool mx_aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -396,16 +454,30 @@ static int mx_dequantize_t(const uint8_t* codes, const uint8_t* scales, int M, i
     return SNF_OK;
 }
 
-// Tiles of 128 x 128 fill the chip from about 128 of them; below that the split kernel's 16 x 64 (or 16 x 16) do better:
-// MEASURED_SPLIT
-static bool mx_split(int M, int N) { return (int64_t)ceil_div(M, 128) * ceil_div(N, 128) < 128; }
+template <int BM, int BN, int WM, int WN, typename T>
+static int mx_tiles(const uint8_t* a, const uint8_t* as, const uint8_t* w, const uint8_t* ws, const float* bias, int M, int N, int chunks,
+                    int act, T* y, hipStream_t st) {
+    constexpr int THREADS = 64 * WM * WN, STAGES = 2 * mx_stage(BM, BN), OUT = WM * WN * 32 * MX_PITCH * 4, LDS = STAGES > OUT ? STAGES : OUT;
+    const int rts = ceil_div(M, BM), cts = ceil_div(N, BN);
+    SNF_REQUIRE(((int64_t)rts * cts + 8) * THREADS < ((int64_t)1 << 32), "snf_mxfp4_linear: %d x %d is too large for one launch", M, N);
+    const auto kernel = k_mxfp4_linear<BM, BN, WM, WN, T>;
+    if (LDS > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        SNF_REQUIRE(e == hipSuccess, "snf_mxfp4_linear: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
+    }
+    const int per = (rts * cts + 7) / 8;
+    kernel<<<dim3(8 * per), dim3(THREADS), LDS, st>>>(a, as, w, ws, bias, M, N, chunks, act, y, rts, cts);
+    SNF_LAUNCH_CHECK("snf_mxfp4_linear");
+    return SNF_OK;
+}
 
 template <typename T>
 static int mx_linear_t(const uint8_t* a, const uint8_t* as, const uint8_t* w, const uint8_t* ws, const float* bias, int M, int K, int N,
                        int act, T* y, hipStream_t st) {
-    constexpr int BM = 128, BN = 128;
     const int chunks = ceil_div(K, 256);
-    if (mx_split(M, N)) {
+    // (tiles of 128 x 128 walk all of k, one workgroup each: few of them leave the chip idle.  512 x 5120 -> 1280, 40 tiles: split 10.0 us,
+    // tiles 18.1; 1024 x 5120 -> 1280, 80 tiles: 21.1 and 18.5; 512 x 1280 -> 5120, 160 tiles: 13.4 and 9.8)
+    if ((int64_t)ceil_div(M, 128) * ceil_div(N, 128) < 64) {
         const int cts = ceil_div(N, 16), mt = M <= 16 ? 1 : M <= 32 ? 2 : 4, rts = ceil_div(M, 16 * mt);
         SNF_REQUIRE((int64_t)rts * cts * 512 < ((int64_t)1 << 32), "snf_mxfp4_linear: %d x %d is too large for one launch", M, N);
         const dim3 grid((unsigned)(rts * cts)), block(512);
@@ -415,12 +487,12 @@ static int mx_linear_t(const uint8_t* a, const uint8_t* as, const uint8_t* w, co
         SNF_LAUNCH_CHECK("snf_mxfp4_linear (split)");
         return SNF_OK;
     }
-    const int rts = ceil_div(M, BM), cts = ceil_div(N, BN);
-    SNF_REQUIRE(((int64_t)rts * cts + 8) * 256 < ((int64_t)1 << 32), "snf_mxfp4_linear: %d x %d is too large for one launch", M, N);
-    const int per = (rts * cts + 7) / 8;
-    k_mxfp4_linear<BM, BN, T><<<dim3(8 * per), dim3(256), 2 * 8 * (BM + BN) * 16, st>>>(a, as, w, ws, bias, M, N, chunks, act, y, rts, cts);
-    SNF_LAUNCH_CHECK("snf_mxfp4_linear");
-    return SNF_OK;
+    // (bytes from the caches halve with tiles of 256 x 256, but one workgroup fills a CU and nothing runs beside its loads and stores:
+    // 16384 x 5120 -> 5120 fp32 243 us against 280, 16384 x 1280 -> 5120 100 against 104, both with 1280 such tiles; with 640 and 320 of
+    // them 8192 x 1280 -> 5120 takes 58 against 52, 4096 x 1280 -> 5120 40 against 32)
+    if ((int64_t)ceil_div(M, 256) * ceil_div(N, 256) >= 1024)
+        return mx_tiles<256, 256, 4, 2, T>(a, as, w, ws, bias, M, N, chunks, act, y, st);
+    return mx_tiles<128, 128, 2, 2, T>(a, as, w, ws, bias, M, N, chunks, act, y, st);
 }
 
 template <typename SRC, typename T>
@@ -482,6 +554,7 @@ int snf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int
 int snf_mxfp4_linear(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* w_codes, const uint8_t* w_scales, const float* bias,
                      int M, int K, int N, int act, void* y, int dtype, snf_stream_t stream) {
     SNF_REQUIRE(M >= 0 && K >= 1 && N >= 1, "snf_mxfp4_linear: bad sizes M=%d K=%d N=%d", M, K, N);
+    SNF_REQUIRE(M < 1 << 28 && N < 1 << 28, "snf_mxfp4_linear: M=%d, N=%d are 2^28 at most", M, N);
     SNF_REQUIRE(act >= SNF_ACT_NONE && act <= SNF_ACT_GELU, "snf_mxfp4_linear: unknown activation %d", act);
     if (M == 0) return SNF_OK;
     SNF_REQUIRE(a_codes && a_scales && w_codes && w_scales && y, "snf_mxfp4_linear: null pointer");
