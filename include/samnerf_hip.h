@@ -549,16 +549,22 @@ int snf_top_distill_bwd(const void* z, int dtype, int R, int V, int64_t ld, cons
  * a block that holds an inf or a NaN has s = 255 and reads back as NaN.  With C = ceil(K / 256):
  *   codes  uint8 [8 C][M][16]   low nibble first (16-byte aligned);   scales uint8 [C][2][M][4]: byte j of (c, h, row) belongs to block
  *   8 c + 2 j + h (4-byte aligned).  The columns from K to 256 C hold zeros.
- * snf_mxfp4_quantize: x [M, K] of `dtype` with rows `ld` elements apart.  snf_mxfp4_dequantize: the values of the codes, out [M, K]
+ * snf_mxfp4_quantize: x [M, K] of `dtype` with rows `ld` elements apart.  snf_mxfp4_quantize_planes: x = hi + lo, the k-blocked bf16 planes
+ *   [K/8][M][8] of snf_layernorm_planes and the like (16-byte aligned).  snf_mxfp4_dequantize: the values of the codes, out [M, K]
  *   contiguous.  snf_mxfp4_linear: y [M, N] of `dtype` = act(a w^T + bias), w quantised from [N, K], bias [N] fp32 or NULL, fp32 sums.
  *   Products below 2^-126 count as zero.  M = 0 is a call without work.
- * snf_mxfp4_linear_rows: the same for up to SNF_MXFP4_ROWS rows x [M, K] of `dtype` (rows `ld` elements apart) that are quantised on the
+ * snf_mxfp4_linear_quantized: the result as the next product's operand, codes and scales of act(a w^T + bias) as snf_mxfp4_quantize would
+ *   make them from its fp32 values; N a multiple of 256.
+ * snf_mxfp4_linear_rows: snf_mxfp4_linear for up to SNF_MXFP4_ROWS rows x [M, K] of `dtype` (rows `ld` elements apart) that are quantised on the
  *   way into the product: one launch.  The same result as snf_mxfp4_quantize followed by snf_mxfp4_linear. */
 #define SNF_MXFP4_ROWS 16
 int snf_mxfp4_quantize(const void* x, int dtype, int M, int K, int64_t ld, uint8_t* codes, uint8_t* scales, snf_stream_t stream);
+int snf_mxfp4_quantize_planes(const uint16_t* hi, const uint16_t* lo, int M, int K, uint8_t* codes, uint8_t* scales, snf_stream_t stream);
 int snf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* out, int dtype, snf_stream_t stream);
 int snf_mxfp4_linear(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* w_codes, const uint8_t* w_scales, const float* bias,
                      int M, int K, int N, int act, void* y, int dtype, snf_stream_t stream);
+int snf_mxfp4_linear_quantized(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* w_codes, const uint8_t* w_scales,
+                               const float* bias, int M, int K, int N, int act, uint8_t* y_codes, uint8_t* y_scales, snf_stream_t stream);
 int snf_mxfp4_linear_rows(const void* x, int dtype, int64_t ld, const uint8_t* w_codes, const uint8_t* w_scales, const float* bias, int M,
                           int K, int N, int act, void* y, int out_dtype, snf_stream_t stream);
 

@@ -160,8 +160,10 @@ SIGNATURES = {
     "snf_top_distill_fwd": [P, I, I, I, c_int64, P, I, P, I, P, I, F, F, P, P, P, P, I, P, P, P, c_int64, P],
     "snf_top_distill_bwd": [P, I, I, I, c_int64, P, I, I, F, F, P, I, P, P, P, P, P, P],
     "snf_mxfp4_quantize": [P, I, I, I, c_int64, P, P, P],
+    "snf_mxfp4_quantize_planes": [P, P, I, I, P, P, P],
     "snf_mxfp4_dequantize": [P, P, I, I, P, I, P],
     "snf_mxfp4_linear": [P, P, P, P, P, I, I, I, I, P, I, P],
+    "snf_mxfp4_linear_quantized": [P, P, P, P, P, I, I, I, I, P, P, P],
     "snf_mxfp4_linear_rows": [P, I, c_int64, P, P, P, I, I, I, I, P, I, P],
     "snf_pixel_indices": [P, I, I, I, I, I, P, P],
     "snf_generate_rays": [P, I, P, P, I, P, P, P, P, P],

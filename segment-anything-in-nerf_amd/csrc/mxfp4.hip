@@ -35,6 +35,26 @@ __device__ __forceinline__ int mx_scale_byte(uint32_t amax_bits) {
 // 2^(byte - 127) as a float (byte < 255; byte 0 is the subnormal 2^-127)
 __device__ __forceinline__ float mx_scale_float(int byte) { return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u); }
 
+// a block that is one lane's: its 16 bytes of codes and its scale byte
+__device__ __forceinline__ uint4 mx_block(const float (&v)[32], int& sb) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    sb = mx_scale_byte(amax);
+    const float sc = mx_scale_float(sb);
+    uint32_t d[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t c = 0;
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i], v[8 * i + 1], sc, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 2], v[8 * i + 3], sc, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 4], v[8 * i + 5], sc, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 6], v[8 * i + 7], sc, 3);
+        d[i] = sb == 255 ? 0x77777777u : c;  // (any non-zero magnitude: NaN under a NaN scale)
+    }
+    return make_uint4(d[0], d[1], d[2], d[3]);
+}
+
 // ---- quantisation ---------------------------------------------------------------------------------------------------------------
 // A workgroup takes 32 rows x 256 columns.  A lane loads 16 bytes of a row (whole rows of the tile are contiguous), the lanes of a block
 // agree on its largest magnitude by cross-lane exchanges, convert their own values and put the codes into LDS in the order of the layout;
@@ -102,6 +122,42 @@ __global__ __launch_bounds__(256) void k_mxfp4_quantize(const T* __restrict__ x,
     }
 }
 
+// The operand planes of the encoder's producers (x = hi + lo, bf16, [K / 8][M][8]) instead of rows: four of their k-blocks are a block.
+// A workgroup takes 64 rows x 256 k; a thread has whole blocks of one row, so nothing is exchanged but the scale bytes.
+__global__ __launch_bounds__(256) void k_mxfp4_quantize_planes(const uint4* __restrict__ hi, const uint4* __restrict__ lo, int M, int K,
+                                                               int chunks, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_scales[2 * 64 * 4];
+    const int c = (int)(blockIdx.x % (unsigned)chunks), lr = threadIdx.x & 63;
+    const int row = (int)(blockIdx.x / (unsigned)chunks) * 64 + lr;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        const int b = p * 4 + (int)(threadIdx.x >> 6), kb = c * 8 + b;
+        float v[32];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint4 h = make_uint4(0, 0, 0, 0), l = h;
+            if (row < M && kb * 4 + g < K / 8) {
+                h = hi[(size_t)(kb * 4 + g) * M + row];
+                l = lo[(size_t)(kb * 4 + g) * M + row];
+            }
+            const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[8 * g + 2 * i] = __uint_as_float(hw[i] << 16) + __uint_as_float(lw[i] << 16);
+                v[8 * g + 2 * i + 1] = __uint_as_float(hw[i] & 0xFFFF0000u) + __uint_as_float(lw[i] & 0xFFFF0000u);
+            }
+        }
+        int sb;
+        const uint4 d = mx_block(v, sb);
+        if (row < M) *reinterpret_cast<uint4*>(codes + ((size_t)kb * M + row) * 16) = d;
+        s_scales[((b & 1) * 64 + lr) * 4 + (b >> 1)] = (uint8_t)sb;
+    }
+    __syncthreads();
+    if (threadIdx.x < 128 && row < M)
+        reinterpret_cast<uint32_t*>(scales)[((size_t)c * 2 + (threadIdx.x >> 6)) * M + row] =
+            reinterpret_cast<const uint32_t*>(s_scales)[threadIdx.x];
+}
+
 // ---- decoding -------------------------------------------------------------------------------------------------------------------
 // The tiles of the quantisation, the other way: codes and scales of 32 rows x 256 columns into LDS, rows out.
 template <typename T, bool WIDE>
@@ -155,11 +211,30 @@ __global__ __launch_bounds__(256) void k_mxfp4_dequantize(const uint8_t* __restr
 }
 
 // ---- product --------------------------------------------------------------------------------------------------------------------
+// nn.GELU (erf form) as max(v, 0) - |v| / 2 erfc(|v| / sqrt 2): nothing cancels.  erfc(x) = e^(-x^2) P(t), t = 1 / (1 + 0.38 x), P a
+// polynomial of degree 9 without a constant, fitted to e^(x^2) erfc(x) on 0 .. 10 by reweighted least squares (relative error 2e-8);
+// in fp32 the result is within 2.4e-7 of the exact one (1 + erff: 4.5e-7, and the epilogue of 4096 x 1280 -> 5120 takes 20 us longer).
+__device__ __forceinline__ float mx_gelu(float v) {
+    const float a = fminf(fabsf(v), 20.f), x = a * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.38f, x, 1.f));
+    float q = 0.0589650683f;
+    q = fmaf(q, t, -0.262271076f);
+    q = fmaf(q, t, 0.36383757f);
+    q = fmaf(q, t, -0.161427662f);
+    q = fmaf(q, t, 0.229999989f);
+    q = fmaf(q, t, 0.138662234f);
+    q = fmaf(q, t, 0.203903109f);
+    q = fmaf(q, t, 0.213919863f);
+    q = fmaf(q, t, 0.214410931f);
+    const float e = __builtin_amdgcn_exp2f(x * x * -1.4426950408889634f);
+    return __builtin_elementwise_maximum(v, 0.f) - 0.5f * a * (q * t * e);
+}
+
 template <int ACT>
 __device__ __forceinline__ float mx_act(float v) {
     if constexpr (ACT == SNF_ACT_RELU) return v > 0.f || v != v ? v : 0.f;
     else if constexpr (ACT == SNF_ACT_SIGMOID) return 1.f / (1.f + expf(-v));
-    else if constexpr (ACT == SNF_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    else if constexpr (ACT == SNF_ACT_GELU) return mx_gelu(v);
     else return v;
 }
 // f with the activation as a constant: one copy of an epilogue each, no branch per element
@@ -187,7 +262,8 @@ template <int BM, int BN, int WM, int WN, typename T>
 __global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_linear(const uint8_t* __restrict__ a, const uint8_t* __restrict__ as,
                                                                const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
                                                                const float* __restrict__ bias, int M, int N, int chunks, int act,
-                                                               T* __restrict__ y, int row_tiles, int col_tiles) {
+                                                               T* __restrict__ y, uint8_t* __restrict__ y_scales, int row_tiles,
+                                                               int col_tiles) {
     constexpr int WAVES = WM * WN, RB = BM / WM / 32, CB = BN / WN / 32;  // 32-row / 32-column blocks of a wave
     // a stage: codes of the rows [8][BM][16], of the columns [8][BN][16], scales of the rows [2][BM][4], of the columns [2][BN][4]
     constexpr int W_AT = 8 * BM * 16, SA_AT = W_AT + 8 * BN * 16, SW_AT = SA_AT + 8 * BM, STAGE = mx_stage(BM, BN);
@@ -291,12 +367,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_linear(const uint8_t* __
     // out, 32 rows x 64 columns at a time through the wave's own piece of LDS.  Element e of a lane: column 8 (e / 4) + 4 half + e % 4 of
     // its 32-column block, row li.
     float* out = reinterpret_cast<float*>(mx_lds) + wave * 32 * PITCH;
-    constexpr int V = MxVec<T>::N, LPR = 64 / V, RPP = 64 / LPR;  // columns a lane stores at once; lanes of a row; rows of a pass
+    constexpr bool CODES = sizeof(T) == 1;
+    constexpr int V = CODES ? 32 : MxVec<T>::N, LPR = 64 / V, RPP = 64 / LPR;  // columns a lane stores at once; lanes of a row; rows of a pass
     const bool wide = N % V == 0;
     mx_with_act(act, [&](auto fixed) {
 #pragma unroll
         for (int j2 = 0; j2 < CB / 2; ++j2) {
-            const int nb = n0 + (wc * CB + 2 * j2) * 32, col = (lane % LPR) * V;
+            // (codes: a lane has a block of a row; neighbouring lanes have neighbouring rows, whose blocks are neighbours in memory)
+            const int nb = n0 + (wc * CB + 2 * j2) * 32, col = (CODES ? half : lane % LPR) * V;
             float b[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) b[e] = bias && nb + col + e < N ? bias[nb + col + e] : 0.f;
@@ -312,20 +390,33 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_linear(const uint8_t* __
                     }
                 __builtin_amdgcn_wave_barrier();
                 const int mb = m0 + (wr * RB + i) * 32;
+                if constexpr (CODES) {  // (N is a multiple of 256)
+                    float v[32];
 #pragma unroll
-                for (int p = 0; p < 32 / RPP; ++p) {
-                    const int row = p * RPP + lane / LPR;
-                    MxVec<T> o;
+                    for (int e = 0; e < 32; ++e) v[e] = mx_act<decltype(fixed)::value>(out[li * PITCH + col + e] + b[e]);
+                    int sb;
+                    const uint4 d = mx_block(v, sb);
+                    const int m = mb + li, kb = (nb + col) >> 5;
+                    if (m < M && nb < N) {
+                        *reinterpret_cast<uint4*>(y + ((size_t)kb * M + m) * 16) = d;
+                        y_scales[(((size_t)(kb >> 3) * 2 + (kb & 1)) * M + m) * 4 + ((kb & 7) >> 1)] = (uint8_t)sb;
+                    }
+                } else {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) o.v[e] = (T)mx_act<decltype(fixed)::value>(out[row * PITCH + col + e] + b[e]);
-                    if (mb + row >= M || nb + col >= N) continue;
-                    T* dst = y + (int64_t)(mb + row) * N + nb + col;
-                    if (wide) {
-                        __builtin_nontemporal_store(__builtin_bit_cast(mx_f32x4, o), reinterpret_cast<mx_f32x4*>(dst));
-                    } else {
+                    for (int p = 0; p < 32 / RPP; ++p) {
+                        const int row = p * RPP + lane / LPR;
+                        MxVec<T> o;
 #pragma unroll
-                        for (int e = 0; e < V; ++e)
-                            if (nb + col + e < N) dst[e] = o.v[e];
+                        for (int e = 0; e < V; ++e) o.v[e] = (T)mx_act<decltype(fixed)::value>(out[row * PITCH + col + e] + b[e]);
+                        if (mb + row >= M || nb + col >= N) continue;
+                        T* dst = y + (int64_t)(mb + row) * N + nb + col;
+                        if (wide) {
+                            __builtin_nontemporal_store(__builtin_bit_cast(mx_f32x4, o), reinterpret_cast<mx_f32x4*>(dst));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < V; ++e)
+                                if (nb + col + e < N) dst[e] = o.v[e];
+                        }
                     }
                 }
                 __builtin_amdgcn_wave_barrier();
@@ -388,22 +479,8 @@ __global__ __launch_bounds__(512) void k_mxfp4_linear_split(const SRC* __restric
                         for (int i = 0; i < V; ++i) v[g * V + i] = col + g * V + i < K ? (float)src[g * V + i] : 0.f;
                     }
                 }
-                uint32_t amax = 0;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-                sx = mx_scale_byte(amax);
-                const float sc = mx_scale_float(sx);
-                uint32_t d[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t c = 0;
-                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i], v[8 * i + 1], sc, 0);
-                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 2], v[8 * i + 3], sc, 1);
-                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 4], v[8 * i + 5], sc, 2);
-                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 6], v[8 * i + 7], sc, 3);
-                    d[i] = sx == 255 ? 0x77777777u : c;
-                }
-                xq = make_int4((int)d[0], (int)d[1], (int)d[2], (int)d[3]);
+                const uint4 d = mx_block(v, sx);
+                xq = make_int4((int)d.x, (int)d.y, (int)d.z, (int)d.w);
             }
             const mx_i32x8 xx = {xq.x, xq.y, xq.z, xq.w, 0, 0, 0, 0};
             acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(xw, xx, acc[t], 4, 4, 0, sw, 0, sx);
@@ -456,7 +533,7 @@ static int mx_dequantize_t(const uint8_t* codes, const uint8_t* scales, int M, i
 
 template <int BM, int BN, int WM, int WN, typename T>
 static int mx_tiles(const uint8_t* a, const uint8_t* as, const uint8_t* w, const uint8_t* ws, const float* bias, int M, int N, int chunks,
-                    int act, T* y, hipStream_t st) {
+                    int act, T* y, uint8_t* y_scales, hipStream_t st) {
     constexpr int THREADS = 64 * WM * WN, STAGES = 2 * mx_stage(BM, BN), OUT = WM * WN * 32 * MX_PITCH * 4, LDS = STAGES > OUT ? STAGES : OUT;
     const int rts = ceil_div(M, BM), cts = ceil_div(N, BN);
     SNF_REQUIRE(((int64_t)rts * cts + 8) * THREADS < ((int64_t)1 << 32), "snf_mxfp4_linear: %d x %d is too large for one launch", M, N);
@@ -466,9 +543,20 @@ static int mx_tiles(const uint8_t* a, const uint8_t* as, const uint8_t* w, const
         SNF_REQUIRE(e == hipSuccess, "snf_mxfp4_linear: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
     }
     const int per = (rts * cts + 7) / 8;
-    kernel<<<dim3(8 * per), dim3(THREADS), LDS, st>>>(a, as, w, ws, bias, M, N, chunks, act, y, rts, cts);
+    kernel<<<dim3(8 * per), dim3(THREADS), LDS, st>>>(a, as, w, ws, bias, M, N, chunks, act, y, y_scales, rts, cts);
     SNF_LAUNCH_CHECK("snf_mxfp4_linear");
     return SNF_OK;
+}
+
+template <typename T>
+static int mx_tiled(const uint8_t* a, const uint8_t* as, const uint8_t* w, const uint8_t* ws, const float* bias, int M, int N, int chunks,
+                    int act, T* y, uint8_t* y_scales, hipStream_t st) {
+    // (bytes from the caches halve with tiles of 256 x 256, but one workgroup fills a CU and nothing runs beside its loads and stores:
+    // 16384 x 5120 -> 5120 fp32 243 us against 280, 16384 x 1280 -> 5120 100 against 104, both with 1280 such tiles; with 640 and 320 of
+    // them 8192 x 1280 -> 5120 takes 58 against 52, 4096 x 1280 -> 5120 40 against 32)
+    if ((int64_t)ceil_div(M, 256) * ceil_div(N, 256) >= 1024)
+        return mx_tiles<256, 256, 4, 2, T>(a, as, w, ws, bias, M, N, chunks, act, y, y_scales, st);
+    return mx_tiles<128, 128, 2, 2, T>(a, as, w, ws, bias, M, N, chunks, act, y, y_scales, st);
 }
 
 template <typename T>
@@ -487,12 +575,7 @@ static int mx_linear_t(const uint8_t* a, const uint8_t* as, const uint8_t* w, co
         SNF_LAUNCH_CHECK("snf_mxfp4_linear (split)");
         return SNF_OK;
     }
-    // (bytes from the caches halve with tiles of 256 x 256, but one workgroup fills a CU and nothing runs beside its loads and stores:
-    // 16384 x 5120 -> 5120 fp32 243 us against 280, 16384 x 1280 -> 5120 100 against 104, both with 1280 such tiles; with 640 and 320 of
-    // them 8192 x 1280 -> 5120 takes 58 against 52, 4096 x 1280 -> 5120 40 against 32)
-    if ((int64_t)ceil_div(M, 256) * ceil_div(N, 256) >= 1024)
-        return mx_tiles<256, 256, 4, 2, T>(a, as, w, ws, bias, M, N, chunks, act, y, st);
-    return mx_tiles<128, 128, 2, 2, T>(a, as, w, ws, bias, M, N, chunks, act, y, st);
+    return mx_tiled(a, as, w, ws, bias, M, N, chunks, act, y, (uint8_t*)nullptr, st);
 }
 
 template <typename SRC, typename T>
@@ -537,6 +620,21 @@ int snf_mxfp4_quantize(const void* x, int dtype, int M, int K, int64_t ld, uint8
     SNF_REQUIRE(false, "snf_mxfp4_quantize: unknown dtype %d", dtype);
 }
 
+int snf_mxfp4_quantize_planes(const uint16_t* hi, const uint16_t* lo, int M, int K, uint8_t* codes, uint8_t* scales, snf_stream_t stream) {
+    SNF_REQUIRE(M >= 0 && K >= 8 && K % 8 == 0, "snf_mxfp4_quantize_planes: bad sizes M=%d K=%d", M, K);
+    if (M == 0) return SNF_OK;
+    SNF_REQUIRE(hi && lo && codes && scales, "snf_mxfp4_quantize_planes: null pointer");
+    SNF_REQUIRE(snf::mx_aligned(hi, 16) && snf::mx_aligned(lo, 16) && snf::mx_aligned(codes, 16) && snf::mx_aligned(scales, 4),
+                "snf_mxfp4_quantize_planes: an operand is not aligned");
+    const int chunks = snf::ceil_div(K, 256);
+    const int64_t blocks = (int64_t)snf::ceil_div(M, 64) * chunks;
+    SNF_REQUIRE(blocks * 256 < ((int64_t)1 << 32), "snf_mxfp4_quantize_planes: %d x %d is too large for one launch", M, K);
+    snf::k_mxfp4_quantize_planes<<<dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream>>>((const uint4*)hi, (const uint4*)lo, M, K, chunks,
+                                                                                               codes, scales);
+    SNF_LAUNCH_CHECK("snf_mxfp4_quantize_planes");
+    return SNF_OK;
+}
+
 int snf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* out, int dtype, snf_stream_t stream) {
     SNF_REQUIRE(M >= 0 && K >= 1, "snf_mxfp4_dequantize: bad sizes M=%d K=%d", M, K);
     if (M == 0) return SNF_OK;
@@ -568,6 +666,19 @@ int snf_mxfp4_linear(const uint8_t* a_codes, const uint8_t* a_scales, const uint
         case SNF_F16: return snf::mx_linear_t(a_codes, a_scales, w_codes, w_scales, bias, M, K, N, act, (_Float16*)y, st);
     }
     SNF_REQUIRE(false, "snf_mxfp4_linear: unknown dtype %d", dtype);
+}
+
+int snf_mxfp4_linear_quantized(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* w_codes, const uint8_t* w_scales,
+                               const float* bias, int M, int K, int N, int act, uint8_t* y_codes, uint8_t* y_scales, snf_stream_t stream) {
+    SNF_REQUIRE(M >= 0 && K >= 1 && N >= 256 && N % 256 == 0, "snf_mxfp4_linear_quantized: bad sizes M=%d K=%d N=%d", M, K, N);
+    SNF_REQUIRE(M < 1 << 28 && N < 1 << 28, "snf_mxfp4_linear_quantized: M=%d, N=%d are 2^28 at most", M, N);
+    SNF_REQUIRE(act >= SNF_ACT_NONE && act <= SNF_ACT_GELU, "snf_mxfp4_linear_quantized: unknown activation %d", act);
+    if (M == 0) return SNF_OK;
+    SNF_REQUIRE(a_codes && a_scales && w_codes && w_scales && y_codes && y_scales, "snf_mxfp4_linear_quantized: null pointer");
+    SNF_REQUIRE(snf::mx_aligned(a_codes, 16) && snf::mx_aligned(w_codes, 16) && snf::mx_aligned(a_scales, 4) && snf::mx_aligned(w_scales, 4) &&
+                    snf::mx_aligned(y_codes, 16) && snf::mx_aligned(y_scales, 4),
+                "snf_mxfp4_linear_quantized: an operand is not aligned");
+    return snf::mx_tiled(a_codes, a_scales, w_codes, w_scales, bias, M, N, snf::ceil_div(K, 256), act, y_codes, y_scales, (hipStream_t)stream);
 }
 
 int snf_mxfp4_linear_rows(const void* x, int dtype, int64_t ld, const uint8_t* w_codes, const uint8_t* w_scales, const float* bias, int M,

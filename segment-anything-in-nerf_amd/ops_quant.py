@@ -7,6 +7,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._opcore import ACT_GELU, ACT_NONE, DTYPE_CODE, _dev, _launch, _p, _rows, _stream_on
+from .ops_vit import Planes
 
 __all__ = ["MXFP4_BLOCK", "Mxfp4", "quantize_mxfp4", "dequantize_mxfp4", "linear_mxfp4"]
 
@@ -56,10 +57,20 @@ class Mxfp4:
         return dequantize_mxfp4(self)
 
 
-def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
-    """x [..., K] (float32 / bfloat16 / float16; rows may be strided) -> Mxfp4.  Per block of 32 along K the scale is
+def _empty(M: int, K: int, dev) -> Tuple[torch.Tensor, torch.Tensor]:
+    chunks = -(-K // 256)
+    return (torch.empty((8 * chunks, M, 16), device=dev, dtype=torch.uint8), torch.empty((2 * chunks, M, 4), device=dev, dtype=torch.uint8))
+
+
+def quantize_mxfp4(x: Union[torch.Tensor, Planes]) -> Mxfp4:
+    """x [..., K] (float32 / bfloat16 / float16; rows may be strided; or the encoder's operand planes) -> Mxfp4.  Per block of 32 along K the scale is
     2^max(floor(log2 max|x|) - 2, -127); values are rounded to the nearest code (halves to even), magnitudes above 6 scales become 6.
     Blocks with an infinity or a NaN become NaN as a whole.  The last block of a K that 32 does not divide is filled with zeros."""
+    if isinstance(x, Planes):
+        dev = _dev(x.hi, "x")
+        codes, scales = _empty(x.M, x.K, dev)
+        _launch("snf_mxfp4_quantize_planes", _p(x.hi), _p(x.lo), x.M, x.K, _p(codes), _p(scales), _stream_on(dev), units=4.0 * x.M * x.K)
+        return Mxfp4._of(codes, scales, x.K, (x.M, x.K))
     if not isinstance(x, torch.Tensor) or x.dtype not in DTYPE_CODE:
         raise TypeError(f"quantize_mxfp4: float32, bfloat16 or float16 expected, got {getattr(x, 'dtype', type(x))}")
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -69,9 +80,7 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
     if x.dim() == 1:
         x = x.unsqueeze(0)
     M = x.numel() // K
-    chunks = -(-K // 256)
-    codes = torch.empty((8 * chunks, M, 16), device=dev, dtype=torch.uint8)
-    scales = torch.empty((2 * chunks, M, 4), device=dev, dtype=torch.uint8)
+    codes, scales = _empty(M, K, dev)
     if M:
         x, ld = _rows(x.detach())
         _launch("snf_mxfp4_quantize", _p(x), DTYPE_CODE[x.dtype], M, K, ld, _p(codes), _p(scales), _stream_on(dev),
@@ -93,11 +102,15 @@ def dequantize_mxfp4(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tens
     return out
 
 
-def linear_mxfp4(x: Union[torch.Tensor, Mxfp4], w: Mxfp4, bias: Optional[torch.Tensor] = None, act: int = ACT_NONE,
-                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """act(x W^T + bias) with both operands in 4 bits and float32 sums: x [..., K] is quantised on the way in (or comes as an Mxfp4),
+def linear_mxfp4(x: Union[torch.Tensor, Mxfp4, Planes], w: Mxfp4, bias: Optional[torch.Tensor] = None, act: int = ACT_NONE,
+                 out_dtype: Optional[torch.dtype] = None, quantized: bool = False) -> Union[torch.Tensor, Mxfp4]:
+    """act(x W^T + bias) with both operands in 4 bits and float32 sums: x [..., K] is quantised on the way in (rows, or the
+    encoder's operand planes) or comes as an Mxfp4,
     w = quantize_mxfp4(weight [N, K]) once per checkpoint, bias [N] float32, act one of ops.ACT_*.  The result [..., N] has x's type
-    (float32 for an Mxfp4) unless out_dtype says otherwise."""
+    (float32 for an Mxfp4 or planes) unless out_dtype says otherwise; quantized=True returns quantize_mxfp4 of the float32 result instead (an operand
+    of the next layer; written by the product itself where N is a multiple of 256)."""
+    if isinstance(x, Planes):
+        x = quantize_mxfp4(x)
     if not isinstance(w, Mxfp4) or len(w.shape) != 2:
         raise TypeError("linear_mxfp4: w is quantize_mxfp4(weight) of a weight [N, K]")
     if not isinstance(x, Mxfp4):
@@ -109,6 +122,10 @@ def linear_mxfp4(x: Union[torch.Tensor, Mxfp4], w: Mxfp4, bias: Optional[torch.T
         raise ValueError("linear_mxfp4: a weight without rows")
     if not ACT_NONE <= int(act) <= ACT_GELU:
         raise ValueError(f"linear_mxfp4: unknown activation {act}")
+    if quantized:
+        if out_dtype not in (None, torch.float32):
+            raise ValueError(f"linear_mxfp4: a quantized result comes from float32, not from {out_dtype}")
+        out_dtype = torch.float32
     if out_dtype is None:
         out_dtype = torch.float32 if isinstance(x, Mxfp4) else x.dtype
     if out_dtype not in DTYPE_CODE:
@@ -120,7 +137,16 @@ def linear_mxfp4(x: Union[torch.Tensor, Mxfp4], w: Mxfp4, bias: Optional[torch.T
         if bias.dtype != torch.float32 or tuple(bias.shape) != (w.M,):
             raise ValueError(f"linear_mxfp4: bias is float32 [{w.M}], got {bias.dtype} {tuple(bias.shape)}")
         bias = bias.contiguous()
-    y = torch.empty(tuple(x.shape[:-1]) + (w.M,), device=dev, dtype=out_dtype)
+    shape = tuple(x.shape[:-1]) + (w.M,)
+    if quantized:
+        q = x if isinstance(x, Mxfp4) else quantize_mxfp4(x)
+        if w.M % 256:
+            return quantize_mxfp4(linear_mxfp4(q, w, bias, act))
+        codes, scales = _empty(q.M, w.M, dev)
+        _launch("snf_mxfp4_linear_quantized", _p(q.codes), _p(q.scales), _p(w.codes), _p(w.scales), _p(bias), q.M, q.K, w.M, int(act),
+                _p(codes), _p(scales), _stream_on(dev), tag=f"{q.K}x{w.M}", units=2.0 * q.M * q.K * w.M)
+        return Mxfp4._of(codes, scales, w.M, shape)
+    y = torch.empty(shape, device=dev, dtype=out_dtype)
     if y.numel() == 0:
         return y
     if isinstance(x, Mxfp4):

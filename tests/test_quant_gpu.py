@@ -289,3 +289,124 @@ def test_refusals_on_the_device():
         C._launch("snf_mxfp4_linear", C._p(w.codes) + 4, C._p(w.scales), C._p(w.codes), C._p(w.scales), None, 3, 64, 8, 0, C._p(x), 0, C._stream())
     with pytest.raises(_lib.SnfError):
         C._launch("snf_mxfp4_linear", C._p(w.codes), C._p(w.scales), C._p(w.codes), C._p(w.scales), None, 3, 64, 8, 9, C._p(x), 0, C._stream())
+
+
+@pytest.mark.parametrize("M,K", [(1, 8), (70, 40), (64, 256), (130, 264), (33, 1280)])
+def test_quantize_planes_vs_rows(M, K):
+    """The encoder's operand planes hold hi + lo: the codes of that sum."""
+    from samnerf_amd import ops
+    x = torch.randn((M, K), generator=torch.Generator().manual_seed(K)) * 3
+    planes = ops.split_planes_kb(x.cuda())
+    q = ops.quantize_mxfp4(planes)
+    check_quantised(planes.float().cpu(), q)
+    w = ops.quantize_mxfp4(torch.randn((9, K), device="cuda"))
+    assert torch.equal(ops.linear_mxfp4(planes, w), ops.linear_mxfp4(q, w))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 256, 32), (5, 40, 64), (37, 512, 100), (130, 256, 1003), (300, 1280, 320), (700, 100, 256), (8200, 8192, 64)])
+def test_linear_quantized_result(M, N, K):
+    """The next layer's operand from the product itself: the codes of its float32 result (the two kernels may add in another order where
+    one deals k out among waves: those sizes are compared by value, to a step of a block's scale)."""
+    from samnerf_amd import ops
+    g = torch.Generator().manual_seed(M + N + K)
+    x, w, b = torch.randn((M, K), generator=g).cuda(), torch.randn((N, K), generator=g).cuda(), torch.randn((N,), generator=g).cuda()
+    wq = ops.quantize_mxfp4(w)
+    xq = ops.quantize_mxfp4(x)
+    for act in (0, 3):
+        q = ops.linear_mxfp4(x.view(M, 1, K), wq, b, act=act, quantized=True)
+        assert isinstance(q, ops.Mxfp4) and q.shape == (M, 1, N)
+        y = ops.linear_mxfp4(xq, wq, b, act=act)
+        want = ops.quantize_mxfp4(y)
+        if -(-M // 128) * -(-N // 128) >= 64 or N % 256:
+            assert torch.equal(q.codes, want.codes) and torch.equal(q.scales, want.scales)
+        else:  # one rounding border crossed moves a value by a code, 2 scales at most; a scale that doubles rounds to twice the step.  The two
+            # sums differ by at most 2 K 2^-24 sum|a w|, under 1e-3 of a block's smallest step (scale / 2): less than 1 % lie that near to one
+            step = y.view(M, -1).abs().amax(dim=1, keepdim=True) / 2
+            assert bool(((q.float().view(M, N) - want.float()).abs() <= step).all())
+            assert float((q.float().view(M, N) != want.float()).float().mean()) <= 0.01
+    e = ops.linear_mxfp4(x[:0], wq, b, quantized=True)
+    assert e.M == 0 and e.shape == (0, N)
+    with pytest.raises(ValueError):
+        ops.linear_mxfp4(x, wq, b, out_dtype=torch.float16, quantized=True)
+
+
+def test_gelu_far_out_and_not_finite():
+    """The activation at both ends: 0 and the value itself; an infinite sum gives its limit, a NaN stays one."""
+    from samnerf_amd import ops
+    w = ops.quantize_mxfp4(torch.ones((1, 32), device="cuda"))
+    x = torch.zeros((9, 32), device="cuda")
+    v = torch.tensor([-40.0, -9.0, -1e-3, 0.0, 1e-3, 9.0, 40.0, 0.0, 0.0], device="cuda")
+    x[:, 0] = 0.0
+    for M in (9, 40, 8200):  # every kernel of the product
+        xs = x.repeat(-(-M // 9), 1)[:M]
+        for i, b in enumerate(v.tolist()[:7]):
+            y = ops.linear_mxfp4(xs, w, torch.full((1,), b, device="cuda"), act=ops.ACT_GELU)
+            want = 0.5 * b * math.erfc(-b / math.sqrt(2.0))
+            assert float((y.double() - want).abs().max()) <= 8 * 2.0 ** -24 * abs(b)
+        for b, want in ((math.inf, math.inf), (-math.inf, 0.0), (math.nan, math.nan)):
+            y = ops.linear_mxfp4(xs, w, torch.full((1,), b, device="cuda"), act=ops.ACT_GELU)
+            assert bool((torch.isnan(y) if math.isnan(want) else y == want).all())
+
+
+# ---- the encoder in this format -------------------------------------------------------------------------------------------------------
+def _small_encoder(embed, depth=2, window=5):
+    from functools import partial
+    from samnerf_amd.image_encoder import ImageEncoderViT
+    torch.manual_seed(embed)
+    enc = ImageEncoderViT(img_size=224, patch_size=16, embed_dim=embed, depth=depth, num_heads=4, mlp_ratio=2.0, out_chans=32, qkv_bias=True,
+                          norm_layer=partial(torch.nn.LayerNorm, eps=1e-6), use_rel_pos=True, window_size=window,
+                          global_attn_indexes=(depth - 1,))
+    with torch.no_grad():
+        for p in enc.parameters():
+            if p.dim() > 1:
+                p.normal_(0, 0.05)
+    return enc.cuda().eval()
+
+
+@pytest.mark.parametrize("embed", [64, 256])  # the plain path and the one on operand planes
+def test_encoder_blocks_compute_what_their_layers_say(embed, monkeypatch):
+    """Every dense layer of every block goes through the product once, in order, with its own quantised weight and bias, and each result
+    is the exact product of its operands to the bound of product_error; the other format is as before afterwards."""
+    from samnerf_amd import ops
+    enc = _small_encoder(embed)
+    x = torch.randn((1, 3, 224, 224), generator=torch.Generator().manual_seed(1)).cuda()
+    split = enc(x)
+    enc.set_linear_format("mxfp4")
+    y = enc(x)
+    layers = [l for blk in enc.blocks for l in (blk.attn.qkv, blk.attn.proj, blk.mlp.lin1, blk.mlp.lin2)]
+    real, seen = ops.linear_mxfp4, []
+
+    def checked(a, w, bias=None, act=0, **kw):
+        r = real(a, w, bias, act, **kw)
+        lin = layers[len(seen)]
+        seen.append(lin)
+        assert bias is lin.bias and torch.equal(w.float(), ops.quantize_mxfp4(lin.weight.detach()).float())
+        q = a if isinstance(a, ops.Mxfp4) else ops.quantize_mxfp4(a)
+        values = r.float() if isinstance(r, ops.Mxfp4) else r
+        if not isinstance(r, ops.Mxfp4):
+            assert product_error(values.reshape(-1, w.M), q.float().view(-1, w.K).cpu().double(), w.float().cpu().double(),
+                                 bias.detach().cpu().double(), act) <= 1.0
+        return r
+
+    monkeypatch.setattr(ops, "linear_mxfp4", checked)
+    z = enc(x)
+    monkeypatch.undo()
+    assert seen == layers and torch.equal(y, z)
+    assert y.shape == split.shape and bool(torch.isfinite(y).all()) and not torch.equal(y, split)
+    enc.set_linear_format("split")
+    assert torch.equal(enc(x), split)
+
+
+def test_encoder_weights_are_requantised_when_written():
+    enc = _small_encoder(64).set_linear_format("mxfp4")
+    x = torch.randn((1, 3, 224, 224), generator=torch.Generator().manual_seed(1)).cuda()
+    a = enc(x)
+    with torch.no_grad():
+        enc.blocks[0].attn.qkv.weight.mul_(0.5)
+    b = enc(x)
+    assert not torch.equal(a, b)
+    with torch.no_grad():
+        enc.blocks[0].attn.qkv.weight.mul_(2.0)
+    assert torch.equal(enc(x), a)
+    with pytest.raises(ValueError):
+        enc.set_linear_format("fp4")
