@@ -74,20 +74,21 @@ def _chk(t: torch.Tensor, name: str, dtype=torch.float32) -> torch.Tensor:
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # SNF_F32, SNF_BF16, SNF_F16
 
 
-def _dev(t: torch.Tensor, name: str, device=None) -> torch.device:
-    """The ROCm device of `t`, which has to be the current one (the launches go to its stream) and `device` when given."""
-    if not t.is_cuda:
+def _dev(t: torch.Tensor, name: str, device: Optional[int] = None) -> int:
+    """Index of the ROCm device of `t`, which has to be the current one (the launches go to its stream).  With `device` (what a first
+    call has returned): `t` has to be there too."""
+    i = t.get_device()
+    if i < 0 or not t.is_cuda:
         raise RuntimeError(f"{name}: expected a ROCm device tensor; the MI355X path has no CPU fallback")
-    if device is not None and t.device != device:
-        raise RuntimeError(f"{name}: on {t.device}, the other operands are on {device}")
-    if t.device.index != torch.cuda.current_device():
-        raise RuntimeError(f"{name}: on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return t.device
+    if device is None:
+        if i != torch.cuda.current_device():
+            raise RuntimeError(f"{name}: on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    elif i != device:
+        raise RuntimeError(f"{name}: on {t.device}, the other operands are on cuda:{device}")
+    return i
 
 
-def _stream_on(device: torch.device):
-    """Raw handle of the current stream of `device` (which _dev has found to be the current device)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+_stream_on = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None  # device index -> raw handle
 
 
 def _rows(t: torch.Tensor):

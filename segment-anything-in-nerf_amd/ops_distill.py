@@ -51,18 +51,18 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     if not 1 <= k <= min(V, TOP_LOGITS_MAX_K):
         raise ValueError(f"top_logits: k={k} is not in 1 .. {min(V, TOP_LOGITS_MAX_K)}")
     t = _temperature(temperature)
-    dev = _dev(logits, "logits")
-    lead = tuple(logits.shape[:-1])
+    di, dev = _dev(logits, "logits"), logits.device
+    lead = logits.shape[:-1]
     ids = torch.empty(lead + (k,), device=dev, dtype=torch.int32)
     vals = torch.empty(lead + (k,), device=dev, dtype=logits.dtype)
     rest = torch.empty(lead, device=dev, dtype=torch.float32)
     R = rest.numel()
     if R:
-        x, ld = _rows((logits.unsqueeze(0) if logits.dim() == 1 else logits).detach())
+        x, ld = _rows(logits.detach() if logits.requires_grad else logits)
         code = DTYPE_CODE[x.dtype]
         nbytes = int(_L().snf_top_logits_workspace_bytes(R, V, k, code))
         ws = _workspace(nbytes, dev)
-        _launch("snf_top_logits", _p(x), code, R, V, ld, k, t, _p(ids), _p(vals), _p(rest), _p(ws), nbytes, _stream_on(dev),
+        _launch("snf_top_logits", _p(x), code, R, V, ld, k, t, _p(ids), _p(vals), _p(rest), _p(ws), nbytes, _stream_on(di),
                 units=float(R * V * x.element_size()))
     return TopLogits(ids, vals, rest)
 
@@ -73,7 +73,7 @@ class _TopDistill(torch.autograd.Function):
     def forward(ctx, student, ids, logits, rest, temperature: float, weight: float, reduction: str):
         dev = student.device
         V, K = int(student.shape[-1]), int(ids.shape[-1])
-        z, ld = _rows(student.unsqueeze(0) if student.dim() == 1 else student)
+        z, ld = _rows(student)
         ids, logits = ids.contiguous(), logits.contiguous()
         rest = rest.contiguous() if rest is not None else None
         R = z.shape[0]
@@ -82,13 +82,13 @@ class _TopDistill(torch.autograd.Function):
         saved = torch.empty((R * (6 + K) + 1,), device=dev, dtype=torch.float32)
         at = saved.data_ptr()
         counted, divisor, rows = at + 4 * R * (4 + K), at + 4 * R * (5 + K), at + 4 * R * (5 + K) + 4
-        loss = torch.empty(tuple(student.shape[:-1]) if per_row else (), device=dev, dtype=torch.float32)
+        loss = torch.empty(student.shape[:-1] if per_row else (), device=dev, dtype=torch.float32)
         if R or not per_row:
             nbytes = int(_L().snf_top_distill_workspace_bytes(R, V, code))
             ws = _workspace(nbytes, dev)
             _launch("snf_top_distill_fwd", _p(z), code, R, V, ld, _p(ids), int(ids.dtype == torch.int64), _p(logits),
                     DTYPE_CODE[logits.dtype], _p(rest), K, temperature, weight, _p(loss) if per_row else rows, counted, at, at + 16 * R,
-                    int(reduction == "mean"), None if per_row else _p(loss), divisor, _p(ws), nbytes, _stream_on(dev),
+                    int(reduction == "mean"), None if per_row else _p(loss), divisor, _p(ws), nbytes, _stream_on(student.get_device()),
                     units=float(R * V * z.element_size()))
         ctx.args = (student.shape, R, V, ld, K, temperature, weight, per_row)
         ctx.save_for_backward(z, ids, saved)
@@ -113,7 +113,7 @@ class _TopDistill(torch.autograd.Function):
             at = saved.data_ptr()
             counted, divisor = at + 4 * R * (4 + K), at + 4 * R * (5 + K)
             _launch("snf_top_distill_bwd", _p(z), DTYPE_CODE[z.dtype], R, V, ld, _p(ids), int(ids.dtype == torch.int64), K, temperature,
-                    weight, _p(g), int(per_row), None if per_row else divisor, counted, at, at + 16 * R, _p(dz), _stream_on(z.device),
+                    weight, _p(g), int(per_row), None if per_row else divisor, counted, at, at + 16 * R, _p(dz), _stream_on(z.get_device()),
                     units=float(2 * R * V * z.element_size()))
         return dz, None, None, None, None, None, None
 
@@ -133,23 +133,28 @@ def top_logits_distill_loss(student: torch.Tensor, ids: torch.Tensor, logits: to
     _logits(student, "student")
     _logits(logits, "logits")
     t = _temperature(temperature)
-    lead = tuple(student.shape[:-1])
+    lead = student.shape[:-1]
     if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"ids: int32 or int64 expected, got {getattr(ids, 'dtype', type(ids))}")
-    if ids.dim() != student.dim() or tuple(ids.shape[:-1]) != lead or not 1 <= ids.shape[-1] <= TOP_LOGITS_MAX_K:
-        raise ValueError(f"ids: {lead} rows of 1 to {TOP_LOGITS_MAX_K} expected, got {tuple(ids.shape)}")
-    if logits.shape != ids.shape:
-        raise ValueError(f"logits: {tuple(ids.shape)} expected, got {tuple(logits.shape)}")
+    shape = ids.shape
+    if len(shape) != student.dim() or shape[:-1] != lead or not 1 <= shape[-1] <= TOP_LOGITS_MAX_K:
+        raise ValueError(f"ids: {tuple(lead)} rows of 1 to {TOP_LOGITS_MAX_K} expected, got {tuple(shape)}")
+    if logits.shape != shape:
+        raise ValueError(f"logits: {tuple(shape)} expected, got {tuple(logits.shape)}")
     if rest is not None:
         if not isinstance(rest, torch.Tensor) or rest.dtype != torch.float32:
             raise TypeError(f"rest: float32 expected, got {getattr(rest, 'dtype', type(rest))}")
-        if tuple(rest.shape) != lead:
-            raise ValueError(f"rest: {lead} expected, got {tuple(rest.shape)}")
+        if rest.shape != lead:
+            raise ValueError(f"rest: {tuple(lead)} expected, got {tuple(rest.shape)}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction: one of {_REDUCTIONS} expected, got {reduction!r}")
-    weight = float(weight)
-    dev = _dev(student, "student")
-    for name, other in (("ids", ids), ("logits", logits), ("rest", rest)):
-        if other is not None:
-            _dev(other, name, dev)
-    return _TopDistill.apply(student, ids, logits.detach(), rest.detach() if rest is not None else None, t, weight, reduction)
+    di = _dev(student, "student")
+    _dev(ids, "ids", di)
+    _dev(logits, "logits", di)
+    if logits.requires_grad:
+        logits = logits.detach()
+    if rest is not None:
+        _dev(rest, "rest", di)
+        if rest.requires_grad:
+            rest = rest.detach()
+    return _TopDistill.apply(student, ids, logits, rest, t, float(weight), reduction)

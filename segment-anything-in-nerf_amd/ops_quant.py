@@ -68,7 +68,7 @@ def quantize_mxfp4(x: Union[torch.Tensor, Planes]) -> Mxfp4:
     Blocks with an infinity or a NaN become NaN as a whole.  The last block of a K that 32 does not divide is filled with zeros."""
     if isinstance(x, Planes):
         dev = _dev(x.hi, "x")
-        codes, scales = _empty(x.M, x.K, dev)
+        codes, scales = _empty(x.M, x.K, x.hi.device)
         _launch("snf_mxfp4_quantize_planes", _p(x.hi), _p(x.lo), x.M, x.K, _p(codes), _p(scales), _stream_on(dev), units=4.0 * x.M * x.K)
         return Mxfp4._of(codes, scales, x.K, (x.M, x.K))
     if not isinstance(x, torch.Tensor) or x.dtype not in DTYPE_CODE:
@@ -76,13 +76,12 @@ def quantize_mxfp4(x: Union[torch.Tensor, Planes]) -> Mxfp4:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"quantize_mxfp4: rows of at least one value expected, got {tuple(x.shape)}")
     dev = _dev(x, "x")
-    shape, K = tuple(x.shape), int(x.shape[-1])
-    if x.dim() == 1:
-        x = x.unsqueeze(0)
+    shape = x.shape
+    K = shape[-1]
     M = x.numel() // K
-    codes, scales = _empty(M, K, dev)
+    codes, scales = _empty(M, K, x.device)
     if M:
-        x, ld = _rows(x.detach())
+        x, ld = _rows(x.detach() if x.requires_grad else x)
         _launch("snf_mxfp4_quantize", _p(x), DTYPE_CODE[x.dtype], M, K, ld, _p(codes), _p(scales), _stream_on(dev),
                 units=float(M * K * x.element_size()))
     return Mxfp4._of(codes, scales, K, shape)
@@ -95,7 +94,7 @@ def dequantize_mxfp4(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tens
     if dtype not in DTYPE_CODE:
         raise TypeError(f"dequantize_mxfp4: float32, bfloat16 or float16 expected, got {dtype}")
     dev = _dev(q.codes, "q")
-    out = torch.empty(q.shape, device=dev, dtype=dtype)
+    out = torch.empty(q.shape, device=q.codes.device, dtype=dtype)
     if q.M:
         _launch("snf_mxfp4_dequantize", _p(q.codes), _p(q.scales), q.M, q.K, _p(out), DTYPE_CODE[dtype], _stream_on(dev),
                 units=float(out.numel() * out.element_size()))
@@ -137,22 +136,22 @@ def linear_mxfp4(x: Union[torch.Tensor, Mxfp4, Planes], w: Mxfp4, bias: Optional
         if bias.dtype != torch.float32 or tuple(bias.shape) != (w.M,):
             raise ValueError(f"linear_mxfp4: bias is float32 [{w.M}], got {bias.dtype} {tuple(bias.shape)}")
         bias = bias.contiguous()
-    shape = tuple(x.shape[:-1]) + (w.M,)
+    shape, place = (*x.shape[:-1], w.M), w.codes.device
     if quantized:
         q = x if isinstance(x, Mxfp4) else quantize_mxfp4(x)
         if w.M % 256:
             return quantize_mxfp4(linear_mxfp4(q, w, bias, act))
-        codes, scales = _empty(q.M, w.M, dev)
+        codes, scales = _empty(q.M, w.M, place)
         _launch("snf_mxfp4_linear_quantized", _p(q.codes), _p(q.scales), _p(w.codes), _p(w.scales), _p(bias), q.M, q.K, w.M, int(act),
                 _p(codes), _p(scales), _stream_on(dev), tag=f"{q.K}x{w.M}", units=2.0 * q.M * q.K * w.M)
         return Mxfp4._of(codes, scales, w.M, shape)
-    y = torch.empty(shape, device=dev, dtype=out_dtype)
+    y = torch.empty(shape, device=place, dtype=out_dtype)
     if y.numel() == 0:
         return y
     if isinstance(x, Mxfp4):
         q = x
     elif y.numel() <= MXFP4_ROWS * w.M:  # few rows: quantised on the way into the product, one launch
-        x, ld = _rows((x.unsqueeze(0) if x.dim() == 1 else x).detach())
+        x, ld = _rows(x.detach() if x.requires_grad else x)
         _launch("snf_mxfp4_linear_rows", _p(x), DTYPE_CODE[x.dtype], ld, _p(w.codes), _p(w.scales), _p(bias), x.shape[0], w.K, w.M, int(act),
                 _p(y), DTYPE_CODE[out_dtype], _stream_on(dev), tag=f"{w.K}x{w.M}", units=2.0 * y.numel() * w.K)
         return y

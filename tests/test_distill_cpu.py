@@ -51,3 +51,41 @@ def test_distill_loss_refusals():
         f(z, ids, top, rest=rest)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         losses.TopLogitsDistillLoss()(z, ops.TopLogits(ids, top, rest))
+
+
+def test_the_library_refuses_before_any_launch():
+    """Argument checks of the C entry points: host code, no device touched."""
+    from samnerf_amd import _lib
+    lib = _lib.load()
+    p = 4096  # an aligned address that is never followed
+
+    def refused(rc, word):
+        assert rc == -1 and word in lib.snf_last_error(), (rc, lib.snf_last_error())
+
+    ok = dict(x=p, dtype=0, R=4, V=64, ld=64, k=3, T=1.0, ids=p, logits=p, rest=p, ws=None, nbytes=0)
+
+    def top(**kw):
+        a = {**ok, **kw}
+        return lib.snf_top_logits(a["x"], a["dtype"], a["R"], a["V"], a["ld"], a["k"], a["T"], a["ids"], a["logits"], a["rest"], a["ws"],
+                                  a["nbytes"], None)
+
+    for kw, word in ((dict(k=0), b"k=0"), (dict(k=65), b"k=65"), (dict(V=400, ld=400, k=257), b"k=257"), (dict(T=0.0), b"temperature"),
+                     (dict(T=float("nan")), b"temperature"), (dict(dtype=3), b"dtype"), (dict(ld=63), b"overlap"), (dict(R=-1), b"sizes"),
+                     (dict(V=1000001, ld=1000001), b"sizes"), (dict(x=None), b"null"), (dict(rest=None), b"null"),
+                     (dict(V=200000, ld=200000), b"workspace"), (dict(R=2 ** 31 - 1, V=2, ld=2, k=1), b"too many")):
+        refused(top(**kw), word)
+    assert top(R=0, x=None) == 0
+    n = lib.snf_top_logits_workspace_bytes(4, 200000, 3, 0)
+    assert n == 4 * 8 * (-(-(200000 + 3) // 32)) and lib.snf_top_logits_workspace_bytes(4, 64, 3, 0) == 0
+
+    def fwd(**kw):
+        a = {**dict(z=p, dtype=0, R=4, V=64, ld=64, ids=p, top_dtype=0, K=3, T=1.0, stats=p, loss=None, divisor=None, nbytes=0), **kw}
+        return lib.snf_top_distill_fwd(a["z"], a["dtype"], a["R"], a["V"], a["ld"], a["ids"], 0, p, a["top_dtype"], None, a["K"], a["T"], 1.0, p,
+                                       p, a["stats"], p, 0, a["loss"], a["divisor"], None, a["nbytes"], None)
+
+    for kw, word in ((dict(K=0), b"K=0"), (dict(K=257), b"K=257"), (dict(T=-1.0), b"temperature"), (dict(top_dtype=4), b"dtype"),
+                     (dict(ld=8), b"overlap"), (dict(z=None), b"null"), (dict(stats=p + 4), b"aligned"), (dict(V=200000, ld=200000), b"workspace"),
+                     (dict(loss=p), b"null")):
+        refused(fwd(**kw), word)
+    refused(lib.snf_top_distill_bwd(p, 0, 4, 64, 64, p, 0, 3, 1.0, 1.0, None, 0, None, p, p, p, p, None), b"null")
+    refused(lib.snf_top_distill_bwd(p, 9, 4, 64, 64, p, 0, 3, 1.0, 1.0, p, 0, None, p, p, p, p, None), b"dtype")

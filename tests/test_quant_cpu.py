@@ -58,3 +58,36 @@ def test_refusals_without_a_device():
         ops.linear_mxfp4(torch.zeros((2, 64)), w, out_dtype=torch.float64)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.linear_mxfp4(torch.zeros((2, 64)), w)
+
+
+def test_the_library_refuses_before_any_launch():
+    """Argument checks of the C entry points: host code, no device touched."""
+    from samnerf_amd import _lib
+    lib = _lib.load()
+    p = 4096  # an aligned address that is never followed
+
+    def refused(rc, word):
+        assert rc == -1 and word in lib.snf_last_error(), (rc, lib.snf_last_error())
+
+    refused(lib.snf_mxfp4_quantize(p, 7, 3, 64, 64, p, p, None), b"dtype")
+    refused(lib.snf_mxfp4_quantize(p, 0, 3, 0, 64, p, p, None), b"sizes")
+    refused(lib.snf_mxfp4_quantize(p, 0, -1, 64, 64, p, p, None), b"sizes")
+    refused(lib.snf_mxfp4_quantize(p, 0, 3, 64, 63, p, p, None), b"overlap")
+    refused(lib.snf_mxfp4_quantize(None, 0, 3, 64, 64, p, p, None), b"null")
+    refused(lib.snf_mxfp4_quantize(p, 0, 3, 64, 64, p + 8, p, None), b"aligned")
+    refused(lib.snf_mxfp4_quantize(p, 0, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31, p, p, None), b"too large")
+    refused(lib.snf_mxfp4_quantize_planes(p, p, 3, 12, p, p, None), b"sizes")
+    refused(lib.snf_mxfp4_quantize_planes(p, p + 2, 3, 16, p, p, None), b"aligned")
+    refused(lib.snf_mxfp4_dequantize(p, p, 3, 64, p, 3, None), b"dtype")
+    refused(lib.snf_mxfp4_dequantize(p, p, 3, 64, None, 0, None), b"null")
+    refused(lib.snf_mxfp4_linear(p, p, p, p, None, 3, 64, 0, 0, p, 0, None), b"sizes")
+    refused(lib.snf_mxfp4_linear(p, p, p, p, None, 3, 64, 8, 4, p, 0, None), b"activation")
+    refused(lib.snf_mxfp4_linear(p, p, p, p, None, 3, 64, 8, 0, p, 5, None), b"dtype")
+    refused(lib.snf_mxfp4_linear(p, p, p, p, None, 1 << 28, 64, 8, 0, p, 0, None), b"2^28")
+    refused(lib.snf_mxfp4_linear(p + 4, p, p, p, None, 3, 64, 8, 0, p, 0, None), b"aligned")
+    refused(lib.snf_mxfp4_linear_quantized(p, p, p, p, None, 3, 64, 40, 0, p, p, None), b"sizes")
+    refused(lib.snf_mxfp4_linear_rows(p, 0, 64, p, p, None, 17, 64, 8, 0, p, 0, None), b"sizes")
+    refused(lib.snf_mxfp4_linear_rows(p, 0, 63, p, p, None, 2, 64, 8, 0, p, 0, None), b"overlap")
+    # calls without work need no memory
+    assert lib.snf_mxfp4_quantize(None, 0, 0, 64, 64, None, None, None) == 0
+    assert lib.snf_mxfp4_linear(None, None, None, None, None, 0, 64, 8, 0, None, 0, None) == 0
