@@ -406,9 +406,24 @@ __global__ __launch_bounds__(THREADS) void k_top_select(const T* __restrict__ x,
     const int granules = (shift + V + E - 1) / E, live = (granules + TD_GROUP - 1) / TD_GROUP;
     const float c = TD_LOG2E / temperature;
     if (threadIdx.x == 0) { s.bound = 0; s.n = 0; }
+    // a thread's first four groups, and later its first four granules of the groups that are read again, stay in registers
+    constexpr int KEEP = 4;
+    float2 kept[KEEP];
+#pragma unroll
+    for (int q = 0; q < KEEP; ++q) {
+        const int i = q * THREADS + (int)threadIdx.x;
+        kept[q] = i < live ? stats[i] : make_float2(TD_NINF, 0.f);
+    }
+    auto each_group = [&](auto f) {
+#pragma unroll
+        for (int q = 0; q < KEEP; ++q) {
+            const int i = q * THREADS + (int)threadIdx.x;
+            if (i < live) f(kept[q], i);
+        }
+        for (int i = KEEP * THREADS + (int)threadIdx.x; i < live; i += THREADS) f(stats[i], i);
+    };
     float own = TD_NINF;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < live; i += THREADS) own = td_max(own, stats[i].x);
+    each_group([&](float2 st, int) { own = td_max(own, st.x); });
     const float top = td_reduce<THREADS, TdMaxOp>(own, s.red);
     bool exact = top != top;
     float bound = 0.f, m = TD_NINF;  // m: the largest element below the bound
@@ -416,12 +431,10 @@ __global__ __launch_bounds__(THREADS) void k_top_select(const T* __restrict__ x,
     if (!exact) {
         bound = td_bound<THREADS>(s, own, k, sets);
         int hits = 0;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < live; i += THREADS) {
-            const float gm = stats[i].x;
-            if (gm >= bound) ++hits;
-            else m = td_max(m, gm);
-        }
+        each_group([&](float2 st, int) {
+            if (st.x >= bound) ++hits;
+            else m = td_max(m, st.x);
+        });
         int incl = hits;
 #pragma unroll
         for (int d = 1; d < WAVE; d <<= 1) {
@@ -437,23 +450,35 @@ __global__ __launch_bounds__(THREADS) void k_top_select(const T* __restrict__ x,
             found += s_count[w];
         }
         if (hits && found <= TD_CAND)
-            for (int i = threadIdx.x; i < live; i += THREADS)
-                if (stats[i].x >= bound) s_list[at++] = i;
+            each_group([&](float2 st, int i) { if (st.x >= bound) s_list[at++] = i; });
         __syncthreads();
         exact = found > TD_CAND;
     }
     const int team = (int)threadIdx.x / TD_GROUP, member = (int)threadIdx.x % TD_GROUP;
+    uint4 again[KEEP];
+    if (!exact) {
+#pragma unroll
+        for (int q = 0; q < KEEP; ++q) {
+            const int l = q * (THREADS / TD_GROUP) + team;
+            if (l < found) again[q] = g[min(s_list[l] * TD_GROUP + member, granules - 1)];
+        }
+    }
     auto sweep = [&](auto f) {
-#pragma unroll 4
-        for (int q = team; q < found; q += THREADS / TD_GROUP) {
-            const int v = s_list[q] * TD_GROUP + member;
-            if (v >= granules) continue;
-            float e_[E];
-            td_unpack<T>(g[v], e_);
+        auto one = [&](const uint4& r, int l) {
+            const int v = s_list[l] * TD_GROUP + member;
+            float x_[E];
+            td_unpack<T>(r, x_);
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if ((unsigned)(v * E + e - shift) < (unsigned)V) f(e_[e], v * E + e - shift);
+                if ((unsigned)(v * E + e - shift) < (unsigned)V) f(x_[e], v * E + e - shift);
+        };
+#pragma unroll
+        for (int q = 0; q < KEEP; ++q) {
+            const int l = q * (THREADS / TD_GROUP) + team;
+            if (l < found) one(again[q], l);
         }
+        for (int l = KEEP * (THREADS / TD_GROUP) + team; l < found; l += THREADS / TD_GROUP)
+            one(g[min(s_list[l] * TD_GROUP + member, granules - 1)], l);
     };
     if (!exact) {
         sweep([&](float v, int p) {
@@ -478,11 +503,7 @@ __global__ __launch_bounds__(THREADS) void k_top_select(const T* __restrict__ x,
     if (n > k) m = td_value((uint32_t)(s.sorted[k] >> 32));
     float sum = 0.f;
     if (m > TD_NINF) {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < live; i += THREADS) {
-            const float2 st = stats[i];
-            if (st.x < bound) sum += st.y * td_term(st.x, m, c);
-        }
+        each_group([&](float2 st, int) { if (st.x < bound) sum += st.y * td_term(st.x, m, c); });
         sweep([&](float v, int) { if (v < bound) sum += td_term(v, m, c); });
     }
     for (int i = k + threadIdx.x; i < n; i += THREADS) sum += td_term(td_value((uint32_t)(s.sorted[i] >> 32)), m, c);
@@ -724,26 +745,39 @@ __global__ __launch_bounds__(256) void k_top_distill_bwd(const T* __restrict__ z
     __shared__ uint32_t s_named[TD_CHUNK / 32 + 1];
     __shared__ int s_id[TD_MAX_K];
     __shared__ float s_p[TD_MAX_K];
+    constexpr int KEEP = 4;
     const int64_t row = blockIdx.x / (unsigned)chunks;
     const int p0 = (int)(blockIdx.x % (unsigned)chunks) * TD_CHUNK, len = min(TD_CHUNK, V - p0);
     const T* zp = z + row * ld + p0;
     T* dp = dz + row * V + p0;
+    // what does not depend on anything is asked for first: the row's scalars, a thread's id and p, its first granules
+    int64_t first_id = -1;
+    float first_p = 0.f;
+    if ((int)threadIdx.x < K) {
+        first_id = td_id(ids, ids_wide, row * K + threadIdx.x);
+        first_p = p[row * K + threadIdx.x];
+    }
+    const int shift = PACKED ? (int)((reinterpret_cast<uintptr_t>(zp) & 15) / sizeof(T)) : 0;
+    const int granules = (shift + len + E - 1) / E;
+    const uint4* zg = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(zp) & ~(uintptr_t)15);
+    uint4 r[KEEP];
+    if (PACKED) {
+#pragma unroll
+        for (int q = 0; q < KEEP; ++q) r[q] = zg[min((int)(q * blockDim.x + threadIdx.x), granules - 1)];
+    }
     const bool live = counted[row] != 0.f;
     const float gs = g[g_per_row ? row : 0] * scale / (divisor ? divisor[0] : 1.f);
     const float c = TD_LOG2E / temperature;
     const float4 st = stats[row];
     const float f = gs * st.y;
     if (live) {
-        for (int i = threadIdx.x; i < TD_CHUNK / 32 + 1; i += blockDim.x) s_named[i] = 0;
+        for (int i = threadIdx.x; i <= (shift + len) / 32; i += blockDim.x) s_named[i] = 0;
         __syncthreads();
-    }
-    const int shift = PACKED ? (int)((reinterpret_cast<uintptr_t>(zp) & 15) / sizeof(T)) : 0;
-    if (live) {
         for (int k = threadIdx.x; k < K; k += blockDim.x) {
-            const int64_t i = td_id(ids, ids_wide, row * K + k) - p0;
+            const int64_t i = (k < (int)blockDim.x ? first_id : td_id(ids, ids_wide, row * K + k)) - p0;
             const bool here = i >= 0 && i < len;
             s_id[k] = here ? (int)i : -1;
-            s_p[k] = p[row * K + k];
+            s_p[k] = k < (int)blockDim.x ? first_p : p[row * K + k];
             if (here) atomicOr(&s_named[(i + shift) >> 5], 1u << ((i + shift) & 31));
         }
         __syncthreads();
@@ -761,28 +795,29 @@ __global__ __launch_bounds__(256) void k_top_distill_bwd(const T* __restrict__ z
         }
     }
     if constexpr (PACKED) {
-        const uint4* zg = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(zp) & ~(uintptr_t)15);
         uint4* dg = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(dp) & ~(uintptr_t)15);
-        const int granules = (shift + len + E - 1) / E;
-        for (int v = threadIdx.x; v < granules; v += blockDim.x) {
-            float x[E];
-            struct alignas(16) { T v[E]; } o;
-            if (live) {
-                td_unpack<T>(zg[v], x);
+        for (int v0 = 0; v0 < granules; v0 += KEEP * blockDim.x) {
+            if (v0 > 0) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) o.v[e] = (T)(f * td_exp2((x[e] - st.x) * c));
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) o.v[e] = (T)0.f;
+                for (int q = 0; q < KEEP; ++q) r[q] = zg[min((int)(v0 + q * blockDim.x + threadIdx.x), granules - 1)];
             }
-            const int b = v * E;
-            const uint32_t bits = live ? s_named[b >> 5] >> (b & 31) & ((1u << E) - 1u) : 0u;
-            if (bits == 0 && b >= shift && b + E <= shift + len) {
-                dg[v] = *reinterpret_cast<const uint4*>(&o);
-            } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (!(bits >> e & 1u) && b + e >= shift && b + e < shift + len) dp[b + e - shift] = o.v[e];
+            for (int q = 0; q < KEEP; ++q) {
+                const int v = v0 + q * blockDim.x + threadIdx.x, b = v * E;
+                if (v >= granules) continue;
+                float x[E];
+                struct alignas(16) { T v[E]; } o;
+                td_unpack<T>(r[q], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o.v[e] = live ? (T)(f * td_exp2((x[e] - st.x) * c)) : (T)0.f;
+                const uint32_t bits = live ? s_named[b >> 5] >> (b & 31) & ((1u << E) - 1u) : 0u;
+                if (bits == 0 && b >= shift && b + E <= shift + len) {
+                    dg[v] = *reinterpret_cast<const uint4*>(&o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (!(bits >> e & 1u) && b + e >= shift && b + e < shift + len) dp[b + e - shift] = o.v[e];
+                }
             }
         }
     } else {
