@@ -955,7 +955,7 @@ int snf_top_logits(const void* x, int dtype, int R, int V, int64_t ld, int k, fl
                    void* workspace, int64_t workspace_bytes, snf_stream_t stream) {
     SNF_REQUIRE(R >= 0 && V >= 1 && V <= SNF_TOP_MAX_V, "snf_top_logits: bad sizes R=%d V=%d", R, V);
     SNF_REQUIRE(k >= 1 && k <= snf::TD_MAX_K && k <= V, "snf_top_logits: k=%d is not in 1 .. min(V, %d)", k, snf::TD_MAX_K);
-    SNF_REQUIRE(temperature > 0.f && temperature < INFINITY, "snf_top_logits: temperature %g", (double)temperature);
+    SNF_REQUIRE(temperature >= FLT_MIN && temperature < INFINITY, "snf_top_logits: temperature %g", (double)temperature);
     SNF_REQUIRE(dtype >= SNF_F32 && dtype <= SNF_F16, "snf_top_logits: unknown dtype %d", dtype);
     if (R == 0) return SNF_OK;
     SNF_REQUIRE(x && ids && logits && rest, "snf_top_logits: null pointer");
@@ -981,7 +981,7 @@ int snf_top_distill_fwd(const void* z, int dtype, int R, int V, int64_t ld, cons
                         int mean, float* loss, float* divisor, void* workspace, int64_t workspace_bytes, snf_stream_t stream) {
     SNF_REQUIRE(R >= 0 && V >= 1 && V <= SNF_TOP_MAX_V, "snf_top_distill_fwd: bad sizes R=%d V=%d", R, V);
     SNF_REQUIRE(K >= 1 && K <= snf::TD_MAX_K, "snf_top_distill_fwd: K=%d is not in 1 .. %d", K, snf::TD_MAX_K);
-    SNF_REQUIRE(temperature > 0.f && temperature < INFINITY, "snf_top_distill_fwd: temperature %g", (double)temperature);
+    SNF_REQUIRE(temperature >= FLT_MIN && temperature < INFINITY, "snf_top_distill_fwd: temperature %g", (double)temperature);
     SNF_REQUIRE(dtype >= SNF_F32 && dtype <= SNF_F16 && top_dtype >= SNF_F32 && top_dtype <= SNF_F16, "snf_top_distill_fwd: unknown dtype");
     SNF_REQUIRE(!loss || divisor, "snf_top_distill_fwd: null pointer");
     hipStream_t st = (hipStream_t)stream;
@@ -1005,7 +1005,7 @@ int snf_top_distill_bwd(const void* z, int dtype, int R, int V, int64_t ld, cons
                         const float* p, void* dz, snf_stream_t stream) {
     SNF_REQUIRE(R >= 0 && V >= 1 && V <= SNF_TOP_MAX_V, "snf_top_distill_bwd: bad sizes R=%d V=%d", R, V);
     SNF_REQUIRE(K >= 1 && K <= snf::TD_MAX_K, "snf_top_distill_bwd: K=%d is not in 1 .. %d", K, snf::TD_MAX_K);
-    SNF_REQUIRE(temperature > 0.f && temperature < INFINITY, "snf_top_distill_bwd: temperature %g", (double)temperature);
+    SNF_REQUIRE(temperature >= FLT_MIN && temperature < INFINITY, "snf_top_distill_bwd: temperature %g", (double)temperature);
     SNF_REQUIRE(dtype >= SNF_F32 && dtype <= SNF_F16, "snf_top_distill_bwd: unknown dtype %d", dtype);
     if (R == 0) return SNF_OK;
     SNF_REQUIRE(z && ids && g && counted && stats && p && dz, "snf_top_distill_bwd: null pointer");

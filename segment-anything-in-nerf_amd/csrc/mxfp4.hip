@@ -297,73 +297,86 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_linear(const uint8_t* __
     static_assert(WAVES % (BM / 64) == 0 && WAVES % (BN / 64) == 0, "a wave's rows");
     const uint32_t off_a = (uint32_t)min(m0 + wave % (BM / 64) * 64 + lane, M - 1) * 16u;
     const uint32_t off_w = (uint32_t)min(n0 + wave % (BN / 64) * 64 + lane, N - 1) * 16u;
-    auto copy = [&](int c, uint8_t* __restrict__ stage) {
-        uint8_t* dst = stage + wave * 1024;
-#pragma unroll
-        for (int p = 0; p < A_PIECES; ++p) {
-            const uint8_t* block = a + ((size_t)c * 8 + (p * WAVES + wave) / (BM / 64)) * M * 16;
-            __builtin_amdgcn_global_load_lds((mx_gptr)(block + off_a), (mx_lptr)(dst + p * WAVES * 1024), 16, 0, 0);
-        }
-#pragma unroll
-        for (int p = 0; p < W_PIECES; ++p) {
-            const uint8_t* block = w + ((size_t)c * 8 + (p * WAVES + wave) / (BN / 64)) * N * 16;
-            __builtin_amdgcn_global_load_lds((mx_gptr)(block + off_w), (mx_lptr)(dst + W_AT + p * WAVES * 1024), 16, 0, 0);
-        }
-#pragma unroll
-        for (int p = 0; p < S_PIECES; ++p) {
-            const int piece = p * WAVES + wave;  // rows' first
+    constexpr int PIECES = A_PIECES + W_PIECES + S_PIECES;
+    auto copy = [&](int p, int c, uint8_t* __restrict__ stage) {  // (p is a constant where this is called)
+        if (p < A_PIECES) {
+            const int piece = p * WAVES + wave;
+            const uint8_t* block = a + ((size_t)c * 8 + piece / (BM / 64)) * M * 16;
+            __builtin_amdgcn_global_load_lds((mx_gptr)(block + off_a), (mx_lptr)(stage + piece * 1024), 16, 0, 0);
+        } else if (p < A_PIECES + W_PIECES) {
+            const int piece = (p - A_PIECES) * WAVES + wave;
+            const uint8_t* block = w + ((size_t)c * 8 + piece / (BN / 64)) * N * 16;
+            __builtin_amdgcn_global_load_lds((mx_gptr)(block + off_w), (mx_lptr)(stage + W_AT + piece * 1024), 16, 0, 0);
+        } else {
+            const int piece = (p - A_PIECES - W_PIECES) * WAVES + wave;  // rows' first
             const bool rows = piece < BM / 32;
             const int at = rows ? piece : piece - BM / 32, h = at / ((rows ? BM : BN) / 64), g = at % ((rows ? BM : BN) / 64);
             const int count = rows ? M : N;
-            const uint8_t* half_ = (rows ? as : ws) + ((size_t)c * 2 + h) * count * 4;
-            __builtin_amdgcn_global_load_lds((mx_gptr)(half_ + (uint32_t)min((rows ? m0 : n0) + g * 64 + lane, count - 1) * 4u),
+            const uint8_t* scales = (rows ? as : ws) + ((size_t)c * 2 + h) * count * 4;
+            __builtin_amdgcn_global_load_lds((mx_gptr)(scales + (uint32_t)min((rows ? m0 : n0) + g * 64 + lane, count - 1) * 4u),
                                              (mx_lptr)(stage + SA_AT + piece * 256), 4, 0, 0);
         }
     };
-    auto multiply = [&](const uint8_t* __restrict__ st) {
-        const uint8_t* fa = st + (half * BM + wr * RB * 32 + li) * 16;
-        const uint8_t* fw = st + W_AT + (half * BN + wc * CB * 32 + li) * 16;
+    // One stage: its products and, between them, the copies of stage c + 1 into the other buffer -- one at a time, since a copy holds its
+    // wave up for some 100 cycles: all of them at the start of a stage leave the matrix cores idle that long (both waves of a SIMD issue
+    // theirs at once).  (The pointers are restricted so that the reads of one buffer are known not to wait for the copies into the other.)
+    auto step = [&](const uint8_t* __restrict__ from, uint8_t* __restrict__ into, int c, auto more) {
+        const uint8_t* fa = from + (half * BM + wr * RB * 32 + li) * 16;
+        const uint8_t* fw = from + W_AT + (half * BN + wc * CB * 32 + li) * 16;
         int sa[RB], sw[CB];
 #pragma unroll
-        for (int i = 0; i < RB; ++i) sa[i] = *reinterpret_cast<const int*>(st + SA_AT + (half * BM + (wr * RB + i) * 32 + li) * 4);
+        for (int i = 0; i < RB; ++i) sa[i] = *reinterpret_cast<const int*>(from + SA_AT + (half * BM + (wr * RB + i) * 32 + li) * 4);
 #pragma unroll
-        for (int j = 0; j < CB; ++j) sw[j] = *reinterpret_cast<const int*>(st + SW_AT + (half * BN + (wc * CB + j) * 32 + li) * 4);
-        // the scale's byte is part of the instruction
+        for (int j = 0; j < CB; ++j) sw[j] = *reinterpret_cast<const int*>(from + SW_AT + (half * BN + (wc * CB + j) * 32 + li) * 4);
+        // fragments a step ahead of their products; the scale's byte is part of the instruction
+        mx_i32x8 xa[2][RB], xw[2][CB];
+        auto fetch = [&](int s, mx_i32x8 (&ra)[RB], mx_i32x8 (&rw)[CB]) {
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+                const int4 q = *reinterpret_cast<const int4*>(fa + (s * 2 * BM + i * 32) * 16);
+                ra[i] = mx_i32x8{q.x, q.y, q.z, q.w, 0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int j = 0; j < CB; ++j) {
+                const int4 q = *reinterpret_cast<const int4*>(fw + (s * 2 * BN + j * 32) * 16);
+                rw[j] = mx_i32x8{q.x, q.y, q.z, q.w, 0, 0, 0, 0};
+            }
+        };
+        fetch(0, xa[0], xw[0]);
 #define MX_STEP(S_)                                                                                                              \
     {                                                                                                                            \
-        mx_i32x8 xa[RB], xw[CB];                                                                                                 \
-        _Pragma("unroll") for (int i = 0; i < RB; ++i) {                                                                         \
-            const int4 q = *reinterpret_cast<const int4*>(fa + ((S_) * 2 * BM + i * 32) * 16);                                   \
-            xa[i] = mx_i32x8{q.x, q.y, q.z, q.w, 0, 0, 0, 0};                                                                    \
+        __builtin_amdgcn_sched_barrier(0);                                                                                       \
+        if ((S_) < 3) fetch((S_) + 1, xa[((S_) + 1) & 1], xw[((S_) + 1) & 1]);                                                   \
+        __builtin_amdgcn_sched_barrier(0);                                                                                       \
+        constexpr int LO = (S_) * PIECES / 4, HI = ((S_) + 1) * PIECES / 4;                                                      \
+        _Pragma("unroll") for (int i = 0; i < RB; ++i) _Pragma("unroll") for (int j = 0; j < CB; ++j) {                          \
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xw[(S_) & 1][j], xa[(S_) & 1][i], acc[i][j], 4, 4, S_,   \
+                                                                        sw[j], S_, sa[i]);                                       \
+            if constexpr (decltype(more)::value) {                                                                               \
+                _Pragma("unroll") for (int p = LO; p < HI; ++p) if ((p - LO) * RB * CB / (HI - LO) == i * CB + j) {              \
+                    __builtin_amdgcn_sched_barrier(0);                                                                           \
+                    copy(p, c + 1, into);                                                                                        \
+                    __builtin_amdgcn_sched_barrier(0);                                                                           \
+                }                                                                                                                \
+            }                                                                                                                    \
         }                                                                                                                        \
-        _Pragma("unroll") for (int j = 0; j < CB; ++j) {                                                                         \
-            const int4 q = *reinterpret_cast<const int4*>(fw + ((S_) * 2 * BN + j * 32) * 16);                                   \
-            xw[j] = mx_i32x8{q.x, q.y, q.z, q.w, 0, 0, 0, 0};                                                                    \
-        }                                                                                                                        \
-        _Pragma("unroll") for (int i = 0; i < RB; ++i) _Pragma("unroll") for (int j = 0; j < CB; ++j) acc[i][j] =                \
-            __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xw[j], xa[i], acc[i][j], 4, 4, S_, sw[j], S_, sa[i]);                \
     }
         MX_STEP(0)
         MX_STEP(1)
         MX_STEP(2)
         MX_STEP(3)
 #undef MX_STEP
-    };
-    // (the pointers are restricted so that the reads of one buffer are known not to wait for the copies into the other)
-    auto step = [&](const uint8_t* __restrict__ from, uint8_t* __restrict__ into, int c) {
-        copy(c + 1, into);
-        multiply(from);
         __builtin_amdgcn_sched_barrier(0);  // (the wait for the copies belongs behind the products)
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (decltype(more)::value) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     };
     uint8_t *const even = mx_lds, *const odd = mx_lds + STAGE;
-    copy(0, even);
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) copy(p, 0, even);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    for (int c = 0; c + 1 < chunks; ++c) step(c & 1 ? odd : even, c & 1 ? even : odd, c);
-    multiply((chunks - 1) & 1 ? odd : even);
-    __syncthreads();
+    for (int c = 0; c + 1 < chunks; ++c) step(c & 1 ? odd : even, c & 1 ? even : odd, c, std::true_type{});
+    step((chunks - 1) & 1 ? odd : even, (chunks - 1) & 1 ? even : odd, chunks - 1, std::false_type{});
     // out, 32 rows x 64 columns at a time through the wave's own piece of LDS.  Element e of a lane: column 8 (e / 4) + 4 half + e % 4 of
     // its 32-column block, row li.
     float* out = reinterpret_cast<float*>(mx_lds) + wave * 32 * PITCH;

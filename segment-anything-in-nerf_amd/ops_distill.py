@@ -1,7 +1,6 @@
 """A teacher's top logits and the distillation loss that reads them (csrc/distill.hip); `samnerf_amd.ops` re-exports everything here."""
 from __future__ import annotations
 
-import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -27,8 +26,8 @@ class TopLogits(NamedTuple):
 
 def _temperature(t) -> float:
     t = float(t)
-    if not (t > 0.0 and math.isfinite(t)):
-        raise ValueError(f"temperature must be positive and finite, got {t}")
+    if not 2.0 ** -126 <= t < 2.0 ** 128:
+        raise ValueError(f"temperature: a positive normal float32 expected, got {t}")
     return t
 
 

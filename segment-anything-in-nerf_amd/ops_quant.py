@@ -20,7 +20,7 @@ class Mxfp4:
 
     codes uint8 [8 C, M, 16] and scales uint8 [2 C, M, 4], C = ceil(K / 256), in the order in which the product reads them (the layout
     stands in include/samnerf_hip.h); `shape` is the shape of the tensor that was quantised.  17 / 32 byte a value."""
-    __slots__ = ("codes", "scales", "M", "K", "shape")
+    __slots__ = ("_data", "_codes", "_scales", "M", "K", "shape")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, K: int, shape: Optional[Tuple[int, ...]] = None):
         chunks = -(-int(K) // 256)
@@ -39,27 +39,44 @@ class Mxfp4:
             n *= d
         if self.shape[-1] != self.K or n != self.M:
             raise ValueError(f"Mxfp4: {self.shape} is not a shape of {self.M} rows of {self.K}")
-        self.codes, self.scales = codes, scales
+        self._data, self._codes, self._scales = codes, codes, scales
 
     @classmethod
-    def _of(cls, codes, scales, K: int, shape) -> "Mxfp4":
-        """What quantize_mxfp4 has just laid out: nothing left to check."""
+    def _new(cls, M: int, K: int, device, shape) -> "Mxfp4":
+        """Room for a matrix: codes and scales in one allocation, which the caller's kernel fills."""
         q = object.__new__(cls)
-        q.codes, q.scales, q.M, q.K, q.shape = codes, scales, codes.shape[1], K, shape
+        q._data = torch.empty((-(-K // 256) * 136 * M,), device=device, dtype=torch.uint8)
+        q._codes = q._scales = None
+        q.M, q.K, q.shape = M, K, shape
         return q
 
     @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            n = -(-self.K // 256)
+            self._codes = self._data[:n * 128 * self.M].view(8 * n, self.M, 16)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            n = -(-self.K // 256)
+            self._scales = self._data[n * 128 * self.M:].view(2 * n, self.M, 4)
+        return self._scales
+
+    def _pointers(self) -> Tuple[int, int]:
+        if self._scales is not None:
+            return self.codes.data_ptr(), self._scales.data_ptr()
+        p = self._data.data_ptr()
+        return p, p + -(-self.K // 256) * 128 * self.M
+
+    @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._data.device
 
     def float(self) -> torch.Tensor:
         """The values as float32, in the shape that was quantised."""
         return dequantize_mxfp4(self)
-
-
-def _empty(M: int, K: int, dev) -> Tuple[torch.Tensor, torch.Tensor]:
-    chunks = -(-K // 256)
-    return (torch.empty((8 * chunks, M, 16), device=dev, dtype=torch.uint8), torch.empty((2 * chunks, M, 4), device=dev, dtype=torch.uint8))
 
 
 def quantize_mxfp4(x: Union[torch.Tensor, Planes]) -> Mxfp4:
@@ -68,9 +85,9 @@ def quantize_mxfp4(x: Union[torch.Tensor, Planes]) -> Mxfp4:
     Blocks with an infinity or a NaN become NaN as a whole.  The last block of a K that 32 does not divide is filled with zeros."""
     if isinstance(x, Planes):
         dev = _dev(x.hi, "x")
-        codes, scales = _empty(x.M, x.K, x.hi.device)
-        _launch("snf_mxfp4_quantize_planes", _p(x.hi), _p(x.lo), x.M, x.K, _p(codes), _p(scales), _stream_on(dev), units=4.0 * x.M * x.K)
-        return Mxfp4._of(codes, scales, x.K, (x.M, x.K))
+        q = Mxfp4._new(x.M, x.K, x.hi.device, (x.M, x.K))
+        _launch("snf_mxfp4_quantize_planes", _p(x.hi), _p(x.lo), x.M, x.K, *q._pointers(), _stream_on(dev), units=4.0 * x.M * x.K)
+        return q
     if not isinstance(x, torch.Tensor) or x.dtype not in DTYPE_CODE:
         raise TypeError(f"quantize_mxfp4: float32, bfloat16 or float16 expected, got {getattr(x, 'dtype', type(x))}")
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -79,12 +96,12 @@ def quantize_mxfp4(x: Union[torch.Tensor, Planes]) -> Mxfp4:
     shape = x.shape
     K = shape[-1]
     M = x.numel() // K
-    codes, scales = _empty(M, K, x.device)
+    q = Mxfp4._new(M, K, x.device, shape)
     if M:
         x, ld = _rows(x.detach() if x.requires_grad else x)
-        _launch("snf_mxfp4_quantize", _p(x), DTYPE_CODE[x.dtype], M, K, ld, _p(codes), _p(scales), _stream_on(dev),
+        _launch("snf_mxfp4_quantize", _p(x), DTYPE_CODE[x.dtype], M, K, ld, *q._pointers(), _stream_on(dev),
                 units=float(M * K * x.element_size()))
-    return Mxfp4._of(codes, scales, K, shape)
+    return q
 
 
 def dequantize_mxfp4(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -93,10 +110,10 @@ def dequantize_mxfp4(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tens
         raise TypeError(f"dequantize_mxfp4: an Mxfp4 expected, got {type(q)}")
     if dtype not in DTYPE_CODE:
         raise TypeError(f"dequantize_mxfp4: float32, bfloat16 or float16 expected, got {dtype}")
-    dev = _dev(q.codes, "q")
-    out = torch.empty(q.shape, device=q.codes.device, dtype=dtype)
+    dev = _dev(q._data, "q")
+    out = torch.empty(q.shape, device=q._data.device, dtype=dtype)
     if q.M:
-        _launch("snf_mxfp4_dequantize", _p(q.codes), _p(q.scales), q.M, q.K, _p(out), DTYPE_CODE[dtype], _stream_on(dev),
+        _launch("snf_mxfp4_dequantize", *q._pointers(), q.M, q.K, _p(out), DTYPE_CODE[dtype], _stream_on(dev),
                 units=float(out.numel() * out.element_size()))
     return out
 
@@ -129,22 +146,22 @@ def linear_mxfp4(x: Union[torch.Tensor, Mxfp4, Planes], w: Mxfp4, bias: Optional
         out_dtype = torch.float32 if isinstance(x, Mxfp4) else x.dtype
     if out_dtype not in DTYPE_CODE:
         raise TypeError(f"linear_mxfp4: the result is float32, bfloat16 or float16, not {out_dtype}")
-    dev = _dev(w.codes, "w")
-    _dev(x.codes if isinstance(x, Mxfp4) else x, "x", dev)
+    dev = _dev(w._data, "w")
+    _dev(x._data if isinstance(x, Mxfp4) else x, "x", dev)
     if bias is not None:
         _dev(bias, "bias", dev)
         if bias.dtype != torch.float32 or tuple(bias.shape) != (w.M,):
             raise ValueError(f"linear_mxfp4: bias is float32 [{w.M}], got {bias.dtype} {tuple(bias.shape)}")
         bias = bias.contiguous()
-    shape, place = (*x.shape[:-1], w.M), w.codes.device
+    shape, place = (*x.shape[:-1], w.M), w._data.device
     if quantized:
         q = x if isinstance(x, Mxfp4) else quantize_mxfp4(x)
         if w.M % 256:
             return quantize_mxfp4(linear_mxfp4(q, w, bias, act))
-        codes, scales = _empty(q.M, w.M, place)
-        _launch("snf_mxfp4_linear_quantized", _p(q.codes), _p(q.scales), _p(w.codes), _p(w.scales), _p(bias), q.M, q.K, w.M, int(act),
-                _p(codes), _p(scales), _stream_on(dev), tag=f"{q.K}x{w.M}", units=2.0 * q.M * q.K * w.M)
-        return Mxfp4._of(codes, scales, w.M, shape)
+        out = Mxfp4._new(q.M, w.M, place, shape)
+        _launch("snf_mxfp4_linear_quantized", *q._pointers(), *w._pointers(), _p(bias), q.M, q.K, w.M, int(act), *out._pointers(),
+                _stream_on(dev), tag=f"{q.K}x{w.M}", units=2.0 * q.M * q.K * w.M)
+        return out
     y = torch.empty(shape, device=place, dtype=out_dtype)
     if y.numel() == 0:
         return y
@@ -152,11 +169,11 @@ def linear_mxfp4(x: Union[torch.Tensor, Mxfp4, Planes], w: Mxfp4, bias: Optional
         q = x
     elif y.numel() <= MXFP4_ROWS * w.M:  # few rows: quantised on the way into the product, one launch
         x, ld = _rows(x.detach() if x.requires_grad else x)
-        _launch("snf_mxfp4_linear_rows", _p(x), DTYPE_CODE[x.dtype], ld, _p(w.codes), _p(w.scales), _p(bias), x.shape[0], w.K, w.M, int(act),
-                _p(y), DTYPE_CODE[out_dtype], _stream_on(dev), tag=f"{w.K}x{w.M}", units=2.0 * y.numel() * w.K)
+        _launch("snf_mxfp4_linear_rows", _p(x), DTYPE_CODE[x.dtype], ld, *w._pointers(), _p(bias), x.shape[0], w.K, w.M, int(act), _p(y),
+                DTYPE_CODE[out_dtype], _stream_on(dev), tag=f"{w.K}x{w.M}", units=2.0 * y.numel() * w.K)
         return y
     else:
         q = quantize_mxfp4(x)
-    _launch("snf_mxfp4_linear", _p(q.codes), _p(q.scales), _p(w.codes), _p(w.scales), _p(bias), q.M, q.K, w.M, int(act), _p(y),
+    _launch("snf_mxfp4_linear", *q._pointers(), *w._pointers(), _p(bias), q.M, q.K, w.M, int(act), _p(y),
             DTYPE_CODE[out_dtype], _stream_on(dev), tag=f"{q.K}x{w.M}", units=2.0 * q.M * q.K * w.M)
     return y

@@ -11,7 +11,7 @@ def test_top_logits_refusals():
     from samnerf_amd import ops
     x = torch.zeros((4, 20))
     for bad in (dict(k=0), dict(k=21), dict(k=3, temperature=0.0), dict(k=3, temperature=float("nan")), dict(k=3, temperature=float("inf")),
-                dict(k=3, temperature=-1.0)):
+                dict(k=3, temperature=-1.0), dict(k=3, temperature=1e-39), dict(k=3, temperature=1e39)):
         with pytest.raises(ValueError):
             ops.top_logits(x, **bad)
     with pytest.raises(ValueError):
@@ -69,7 +69,7 @@ def test_the_library_refuses_before_any_launch():
         return lib.snf_top_logits(a["x"], a["dtype"], a["R"], a["V"], a["ld"], a["k"], a["T"], a["ids"], a["logits"], a["rest"], a["ws"],
                                   a["nbytes"], None)
 
-    for kw, word in ((dict(k=0), b"k=0"), (dict(k=65), b"k=65"), (dict(V=400, ld=400, k=257), b"k=257"), (dict(T=0.0), b"temperature"),
+    for kw, word in ((dict(k=0), b"k=0"), (dict(k=65), b"k=65"), (dict(V=400, ld=400, k=257), b"k=257"), (dict(T=0.0), b"temperature"), (dict(T=1e-39), b"temperature"),
                      (dict(T=float("nan")), b"temperature"), (dict(dtype=3), b"dtype"), (dict(ld=63), b"overlap"), (dict(R=-1), b"sizes"),
                      (dict(V=1000001, ld=1000001), b"sizes"), (dict(x=None), b"null"), (dict(rest=None), b"null"),
                      (dict(V=200000, ld=200000), b"workspace"), (dict(R=2 ** 31 - 1, V=2, ld=2, k=1), b"too many")):

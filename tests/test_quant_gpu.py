@@ -209,6 +209,29 @@ def test_linear_vs_reference(M, N, K, dtype):
         assert y.dtype == od and product_error(y, xv, wv, bias.double(), 0) <= 1.0
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K,act", [(8200, 8180, 300, 3), (8192, 8192, 64, 0), (8449, 7937, 257, 1), (1025, 1100, 700, 3), (2000, 1031, 96, 2)])
+def test_linear_tiles_vs_reference(M, N, K, act, dtype):
+    """Sizes that the two tile kernels take, whole tiles and ragged ones: against the decoded operands' product in 64 bits."""
+    from samnerf_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    x = torch.randn((M, K), generator=g, device="cuda").to(dtype)
+    wq = ops.quantize_mxfp4(torch.randn((N, K), generator=g, device="cuda") / math.sqrt(K))
+    bias = torch.randn((N,), generator=g, device="cuda")
+    xq = ops.quantize_mxfp4(x)
+    y = ops.linear_mxfp4(x, wq, bias, act=act)
+    xv, wt = xq.float().double(), wq.float().double().t().contiguous()
+    s = xv @ wt + bias.double()
+    mag = xv.abs() @ wt.abs() + bias.double().abs()
+    exact = act64(s, act)
+    tol = (K + 1) * 2.0 ** -24 * mag * 1.13  # (as product_error)
+    if act in (2, 3):
+        tol += 8 * 2.0 ** -24 * torch.maximum(exact.abs(), s.abs() if act == 3 else torch.ones_like(s))
+    fi = torch.finfo(dtype)
+    tol = tol * (1 + fi.eps) + exact.abs() * fi.eps / 2 + fi.smallest_normal * fi.eps
+    assert bool(((y.double() - exact).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 640, 320), (50, 70, 320), (200, 130, 4100)])
 def test_linear_scales_far_apart(M, N, K):
     """Blocks whose scales differ by up to 2^40 on both sides, and rows of zeros."""
@@ -238,11 +261,11 @@ def test_linear_strided_input_and_views(M):
     assert torch.equal(ops.linear_mxfp4(x, w, big[::4]), ops.linear_mxfp4(x, w, big[::4].clone()))
 
 
-@pytest.mark.parametrize("M", [1, 30, 200])
-def test_linear_repeats_streams_and_graphs(M):
+@pytest.mark.parametrize("M,N", [(1, 300), (30, 300), (1100, 1111), (8200, 8180)])
+def test_linear_repeats_streams_and_graphs(M, N):
     """The same bits again, on another stream, and from a replayed graph with new inputs."""
     from samnerf_amd import ops
-    K, N = 1300, 300
+    K = 1300 if M < 8000 else 300
     w = ops.quantize_mxfp4(torch.randn((N, K), device="cuda"))
     xs = [torch.randn((M, K), device="cuda") for _ in range(3)]
     want = [ops.linear_mxfp4(x, w, act=ops.ACT_GELU) for x in xs]
