@@ -128,7 +128,8 @@ def top_logits_distill_loss(student: torch.Tensor, ids: torch.Tensor, logits: to
     against the student's mass on all places that the ids do not name; without it the teacher's probabilities sum to 1 over the list.
     reduction "mean": over the rows with a target (a row without entries, or whose teacher has no mass, has none; no such row: 0); "sum";
     "none": [...] float32.  An id named twice counts twice for the teacher; an id >= V makes its row NaN.  The teacher's tensors get no
-    gradient.  K <= 256."""
+    gradient.  K <= 256.  (To capture the backward pass into a graph, let no eager graph of the same leaves live: autograd would
+    accumulate on that graph's stream.)"""
     _logits(student, "student")
     _logits(logits, "logits")
     t = _temperature(temperature)

@@ -124,7 +124,7 @@ def linear_mxfp4(x: Union[torch.Tensor, Mxfp4, Planes], w: Mxfp4, bias: Optional
     encoder's operand planes) or comes as an Mxfp4,
     w = quantize_mxfp4(weight [N, K]) once per checkpoint, bias [N] float32, act one of ops.ACT_*.  The result [..., N] has x's type
     (float32 for an Mxfp4 or planes) unless out_dtype says otherwise; quantized=True returns quantize_mxfp4 of the float32 result instead (an operand
-    of the next layer; written by the product itself where N is a multiple of 256)."""
+    of the next layer; written by the product itself where N is a multiple of 256).  No gradient flows through it."""
     if isinstance(x, Planes):
         x = quantize_mxfp4(x)
     if not isinstance(w, Mxfp4) or len(w.shape) != 2:
