@@ -166,8 +166,8 @@ struct TdPart {
 //   long rows: k_top_groups streams them -- any number of workgroups a row, nothing exchanged between waves -- and leaves the maximum and
 //     the sum of exponentials of every 128 bytes; k_top_select, one workgroup a row, finds the bound among the maxima and reads again only
 //     the groups that reach it (about 1.4 k of them: 9 % of a row of 65536 bf16 at k = 64; the groups' results are 6 %).
-// Rows with a NaN and rows where more than TD_CAND elements reach the bound (long runs of equal logits) take the exact way, from memory:
-// bisection of the k-th key over its bits, then of the places among its equals.
+// Rows with a NaN and rows where more than TD_CAND elements reach the bound (long runs of equal logits, sorted rows) take the exact way,
+// from memory (td_select_exact).
 constexpr int TD_CAND = 1024;
 constexpr int TD_GROUP = 8;  // 16-byte granules of a group (td_reduce8)
 
@@ -231,67 +231,114 @@ __device__ __forceinline__ void td_rank(TdSelect<THREADS>& s, int k, int32_t* __
     __syncthreads();
 }
 
-// the elements of a row from memory
-template <typename T, int THREADS, typename F>
-__device__ __forceinline__ void td_scan(const T* p, int len, F f) {
-    constexpr int E = 16 / (int)sizeof(T);
-    const int shift = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
-    const uint4* g = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
-    const int granules = (shift + len + E - 1) / E;
-#pragma unroll 1
-    for (int v = (int)threadIdx.x; v < granules; v += THREADS) {
+__device__ __forceinline__ float td_lse(float m, float sum, float temperature) {
+    return m == INFINITY || m == TD_NINF ? m : m / temperature + logf(sum);
+}
+
+// elements of a row from memory, in the order of their places: all of them, or those of the listed groups (in rising order)
+template <typename T>
+struct TdSlots {
+    static constexpr int E = 16 / (int)sizeof(T);
+    const uint4* g;
+    const int* list;
+    int shift, V, granules, slots;
+    __device__ __forceinline__ TdSlots(const T* p, int V_, const int* list_, int listed) : list(list_), V(V_) {
+        shift = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+        g = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
+        granules = (shift + V + E - 1) / E;
+        slots = list ? listed * TD_GROUP : granules;
+    }
+    template <typename F>
+    __device__ __forceinline__ void one(int slot, F f) const {
+        const int v = list ? list[slot / TD_GROUP] * TD_GROUP + slot % TD_GROUP : slot;
+        if (v >= granules) return;
         float x[E];
         td_unpack<T>(g[v], x);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int at = v * E + e - shift;
-            if ((unsigned)at < (unsigned)len) f(x[e], at);
+            if ((unsigned)at < (unsigned)V) f(x[e], at);
         }
     }
-}
+    template <int THREADS, typename F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll 1
+        for (int slot = (int)threadIdx.x; slot < slots; slot += THREADS) one(slot, f);
+    }
+};
 
-__device__ __forceinline__ float td_lse(float m, float sum, float temperature) {
-    return m == INFINITY || m == TD_NINF ? m : m / temperature + logf(sum);
-}
-
-// the exact way; returns the rest's log-sum-exp
+// The exact way.  `in` holds every element whose key is at least `from` (0: not known), at least k of them; groups whose maximum is below
+// `bound` are in `stats` instead where that is given.  The k-th key is `from` itself where fewer than k lie above it (long runs of equal
+// logits: a few passes over `in`; 4096 rows of 65536 equal bf16, k = 64: 0.90 ms, 4.70 by bisection), else found by bisection of its bits
+// (the same rows ascending: 0.57 ms over the listed groups, 4.57 over all; with a NaN, over all: 3.3 ms); equals of the k-th are taken in
+// the order of their places, which ends as soon as there are enough.  Leaves the k keys in s (for td_rank), returns the rest's log-sum-exp.
 template <typename T, int THREADS>
-__device__ __noinline__ float td_select_exact(TdSelect<THREADS>& s, const T* src, int V, int k, float temperature, int32_t* ids, T* logits) {
+__device__ __noinline__ float td_select_exact(TdSelect<THREADS>& s, const TdSlots<T> in, uint32_t from, const float2* stats, int groups,
+                                              float bound, int k, float temperature) {
     const float c = TD_LOG2E / temperature;
+    int* red = reinterpret_cast<int*>(s.red);
     auto count = [&](auto pred) {
         int n = 0;
-        td_scan<T, THREADS>(src, V, [&](float v, int p) { n += pred(td_key(v), p); });
-        return td_reduce<THREADS, TdCountOp>(n, reinterpret_cast<int*>(s.red));
+        in.template each<THREADS>([&](float v, int) { n += pred(td_key(v)); });
+        return td_reduce<THREADS, TdCountOp>(n, red);
     };
-    uint32_t kth = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t t = kth | 1u << bit;
-        if (count([&](uint32_t key, int) { return key >= t; }) >= k) kth = t;
+    uint32_t kth = from;
+    int above = from ? count([&](uint32_t key) { return key > from; }) : k;
+    if (above >= k) {
+        kth = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t t = kth | 1u << bit;
+            if (count([&](uint32_t key) { return key >= t; }) >= k) kth = t;
+        }
+        above = count([&](uint32_t key) { return key > kth; });
     }
-    const int need = k - count([&](uint32_t key, int) { return key > kth; });
-    const int equal = count([&](uint32_t key, int) { return key == kth; });
-    int cut = V;  // the smallest place with `need` equals before it
-    for (int lo = 0; need < equal && lo < cut;) {
-        const int mid = (lo + cut) >> 1;
-        if (count([&](uint32_t key, int p) { return key == kth && p < mid; }) >= need) cut = mid;
-        else lo = mid + 1;
-    }
+    const int need = k - above, equal = count([&](uint32_t key) { return key == kth; });
     __syncthreads();
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
-    td_scan<T, THREADS>(src, V, [&](float v, int p) {
-        const uint32_t key = td_key(v);
-        if (key > kth || (key == kth && p < cut)) s.key[atomicAdd(&s.n, 1)] = (uint64_t)key << 32 | (uint32_t)~p;
-    });
-    __syncthreads();
-    td_rank<THREADS>(s, k, ids, logits);
     float m = equal > need ? td_value(kth) : TD_NINF, sum = 0.f;
-    if (equal == need) {
-        td_scan<T, THREADS>(src, V, [&](float v, int) { if (td_key(v) < kth) m = td_max(m, v); });
-        m = td_reduce<THREADS, TdMaxOp>(m, s.red);
+    in.template each<THREADS>([&](float v, int p) {
+        const uint32_t key = td_key(v);
+        if (key > kth) s.key[atomicAdd(&s.n, 1)] = (uint64_t)key << 32 | (uint32_t)~p;
+        else if (key < kth) m = td_max(m, v);
+    });
+    int taken = 0;
+    for (int base = 0; base < in.slots && taken < need; base += THREADS) {
+        const int slot = base + (int)threadIdx.x;
+        int mine = 0;
+        if (slot < in.slots) in.one(slot, [&](float v, int) { mine += td_key(v) == kth; });
+        int incl = mine;
+#pragma unroll
+        for (int d = 1; d < WAVE; d <<= 1) {
+            const int t = __shfl_up(incl, d, WAVE);
+            if (lane_id() >= d) incl += t;
+        }
+        if (lane_id() == WAVE - 1) red[threadIdx.x >> 6] = incl;
+        __syncthreads();
+        int at = taken + incl - mine;
+#pragma unroll 1
+        for (int w = 0; w < THREADS / WAVE; ++w) {
+            at += w < (int)(threadIdx.x >> 6) ? red[w] : 0;
+            taken += red[w];
+        }
+        __syncthreads();
+        if (mine && at < need)
+            in.one(slot, [&](float v, int p) {
+                if (td_key(v) == kth && at++ < need) s.key[atomicAdd(&s.n, 1)] = (uint64_t)kth << 32 | (uint32_t)~p;
+            });
     }
-    td_scan<T, THREADS>(src, V, [&](float v, int) { if (td_key(v) < kth) sum += td_term(v, m, c); });
-    sum = td_reduce<THREADS, TdSumOp>(sum, s.red) + (float)(equal - need);
+    __syncthreads();
+    auto others = [&](auto f) {
+        if (stats)
+            for (int i = threadIdx.x; i < groups; i += THREADS)
+                if (stats[i].x < bound) f(stats[i]);
+    };
+    others([&](float2 st) { m = td_max(m, st.x); });
+    m = td_reduce<THREADS, TdMaxOp>(m, s.red);
+    others([&](float2 st) { sum += st.y * td_term(st.x, m, c); });
+    in.template each<THREADS>([&](float v, int) { if (td_key(v) < kth) sum += td_term(v, m, c); });
+    sum = td_reduce<THREADS, TdSumOp>(sum, s.red);
+    if (equal > need) sum += (float)(equal - need) * td_term(td_value(kth), m, c);  // (else kth may be far above m)
     return td_lse(m, sum, temperature);
 }
 
@@ -329,7 +376,9 @@ __global__ __launch_bounds__(THREADS) void k_top_logits(const T* __restrict__ x,
         exact = s.n > Sel::CAND;
     }
     if (exact) {
-        const float r = td_select_exact<T, THREADS>(s, src, V, k, temperature, ids, logits);
+        const float r = td_select_exact<T, THREADS>(s, TdSlots<T>(src, V, nullptr, 0), top != top ? 0u : td_key(bound), nullptr, 0, bound, k,
+                                                    temperature);
+        td_rank<THREADS>(s, k, ids, logits);
         if (threadIdx.x == 0) rest[row] = r;
         return;
     }
@@ -493,7 +542,21 @@ __global__ __launch_bounds__(THREADS) void k_top_select(const T* __restrict__ x,
         exact = s.n > Sel::CAND;
     }
     if (exact) {
-        const float r = td_select_exact<T, THREADS>(s, src, V, k, temperature, ids, logits);
+        const bool listed = top == top && found <= TD_CAND;
+        if (listed) {  // in rising order
+            int* order = reinterpret_cast<int*>(s.sorted);
+            for (int i = threadIdx.x; i < found; i += THREADS) {
+                int rank = 0;
+                for (int j = 0; j < found; ++j) rank += s_list[j] < s_list[i];
+                order[rank] = s_list[i];
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < found; i += THREADS) s_list[i] = order[i];
+            __syncthreads();
+        }
+        const float r = td_select_exact<T, THREADS>(s, TdSlots<T>(src, V, listed ? s_list : nullptr, found), top != top ? 0u : td_key(bound),
+                                                    listed ? stats : nullptr, live, bound, k, temperature);
+        td_rank<THREADS>(s, k, ids, logits);
         if (threadIdx.x == 0) rest[row] = r;
         return;
     }

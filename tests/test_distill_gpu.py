@@ -79,6 +79,31 @@ def test_top_logits_infinities_nan_and_masks(V, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,k", [(60, 7), (3000, 40), (70001, 130), (300000, 256)])
+def test_top_logits_runs_with_gaps(V, k, dtype):
+    """Runs of equal logits around the k-th, between far lower ones and a NaN: nothing of the top reaches the rest's reference."""
+    from samnerf_amd import ops
+    g = torch.Generator().manual_seed(V)
+    high = 600.0 if dtype == torch.float16 else 2000.0
+    x = torch.randn((7, V), generator=g)
+    x[0, V // 3:V // 3 + k] = high                       # exactly k equals, the rest far below
+    x[1, V // 3:V // 3 + k - 1] = high                   # ... beside a NaN: k together
+    x[1, 2] = math.nan
+    x[2, V // 2:] = high                                 # one run that is longer than k, at the end
+    x[3, torch.randperm(V, generator=g)[:V // 2]] = high  # scattered equals
+    x[3, V - 1] = 2 * high
+    x[4] = torch.sort(x[4]).values                       # ascending: the last groups
+    x[5, :V // 2] = -math.inf                            # only a run behind masked places
+    x[5, V // 2:] = -high
+    x[6] = torch.relu(x[6] - 2.0)                        # few different values, most equal
+    x = x.to(dtype)
+    check_top(x, k, 1.0, ops.top_logits(x.cuda(), k))
+    buf = torch.full((7, V + 5), math.inf, dtype=dtype, device="cuda")
+    buf[:, 3:V + 3] = x.cuda()
+    check_top(x, k, 1.0, ops.top_logits(buf[:, 3:V + 3], k))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_top_logits_rows_at_any_address(dtype):
     """Strided rows that start anywhere in a 16-byte granule; what lies between them is never taken."""
     from samnerf_amd import ops
