@@ -423,6 +423,58 @@ def test_distill_repeats_streams_and_graphs(R, V):
         assert all(torch.equal(a, b) for a, b in zip(t2, tops[i]))
 
 
+def classes64(z, ids, top, rest, T):
+    """Of rows whose ids are all entries, in float64: the teacher's mass per place [R, V] and of the rest [R], q [R, V], which are named."""
+    R, V = z.shape
+    a = top.double() / T
+    lse = torch.logsumexp(a if rest is None else torch.cat([a, rest.double()[:, None]], 1), 1, keepdim=True)
+    p = torch.zeros((R, V), dtype=torch.float64).scatter_add_(1, ids.long(), torch.exp(a - lse))
+    pr = torch.exp(rest.double() - lse[:, 0]) if rest is not None else torch.zeros(R, dtype=torch.float64)
+    named = torch.zeros((R, V), dtype=torch.bool).scatter_(1, ids.long(), True)
+    return p, pr, torch.softmax(z.double() / T, 1), named
+
+
+def check_digits(z, ids, top, rest, T):
+    """Bounds that follow the result, also where a row's loss is small.  With d = log p - log q the loss is a sum of p d + q - p over the
+    classes, and an error of d counts by p - q (where |d| > 1/2 by p or q, at most 2.6 |p - q|).  d is off by 8 steps of 2^-24 of the
+    logits over T, and by what the sums are off: 64 places a lane in turn, a tree, some thousand parts joined by lanes, exponentials of
+    exponents up to 30 (3 steps each): 160 + 90 steps.  Probabilities in p d + q - p: the same, at most 6 times the term."""
+    from samnerf_amd import ops
+    p, pr, q, named = classes64(z, ids, top, rest, T)
+    rows, _ = loss64(z.double(), ids, top.double(), rest.double() if rest is not None else None, T)
+    pn, qn = p.sum(1), (q * named).sum(1)
+    qr = (q * ~named).sum(1)
+    size = (z.double().abs().max(1).values + top.double().abs().max(1).values) / T + (rest.double().abs() if rest is not None else 0)
+    steps = 250 + 8 * size
+    apart = ((p - q) * named).abs().sum(1) + (pr - qr).abs()
+    x = z.cuda().requires_grad_(True)
+    got = ops.top_logits_distill_loss(x, ids.cuda(), top.cuda(), rest=rest.cuda() if rest is not None else None, temperature=T, reduction="none")
+    (dx,) = torch.autograd.grad(got, x, torch.ones_like(got))
+    off = (got.detach().cpu().double() - rows).abs()
+    tol = T * T * U * steps * (2.6 * apart + 6 * rows / (T * T))
+    assert bool((off <= tol).all()), (off / tol).max()
+    # a place that is not named: (p_named - q_named) q / q_rest, the two sums off by `steps` of themselves, the exponential of (z - m) / T by
+    # 3 steps of its exponent; then the result's own rounding
+    fi = torch.finfo(z.dtype)
+    share = q / qr.clamp_min(1e-300)[:, None]
+    want = T * (q - (pr[:, None] * share if rest is not None else 0))
+    far = 3 * (z.double().max(1, keepdim=True).values - z.double()) / T + 8
+    gtol = T * share * U * ((steps * (pn + qn))[:, None] if rest is not None else steps[:, None] * qr[:, None]) + want.abs() * (U * far + fi.eps / 2 * 1.01)
+    bad = ((dx.cpu().double() - want).abs() > gtol + fi.smallest_normal * fi.eps) & ~named
+    assert not bool(bad.any()), ((dx.cpu().double() - want).abs() / gtol)[bad].max()
+    return dx.cpu().double(), p, q, named, steps
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [700, 5003, 40000, 100000])
+@pytest.mark.parametrize("k", [1, 2, 8])
+def test_distill_short_list_of_a_long_row(k, V, dtype):
+    """The list holds little of the mass on both sides: rest against rest is a quotient of two numbers close to 1."""
+    for T in (2.0, 4.0):
+        for R in (1, 24):
+            check_digits(*make(R, V, k, dtype, V + k + R, empty=0, T=T), T)
+
+
 def test_refusals_at_the_library():
     from samnerf_amd import _lib
     from samnerf_amd import _opcore as C
