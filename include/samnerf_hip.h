@@ -524,7 +524,7 @@ int snf_attention_planes_rp(const float* qkv, const float* rel_pos_h, const floa
  *   sum of q over the places that the row's ids do not name:
  *     rows[r] = weight T^2 ( sum_k p_k (log p_k - log q_ids_k) + p_rest (log p_rest - log q_rest) )
  *   without rest, p sums to 1 over the entries.  Rows without an entry, or whose teacher has no mass, are no targets: rows = counted = 0.
- *   An id >= V makes its row NaN.  stats [R, 4] (16-byte aligned) and p [R, K] are kept for the backward pass.  loss (or NULL) [1] = sum of
+ *   An id >= V makes its row NaN.  stats [R, 2] (8-byte aligned) and diff [R, K] are kept for the backward pass.  loss (or NULL) [1] = sum of
  *   rows / divisor[0], divisor [1] = number of counted rows (at least 1) or, mean == 0, 1.  workspace:
  *   snf_top_distill_workspace_bytes(...) bytes, 8-byte aligned.
  * snf_top_distill_bwd: dz [R, V] contiguous of `dtype` = g weight T (q_v - sum_{k: ids_k = v} p_k - (v not named) p_rest q_v / q_rest),
@@ -536,11 +536,11 @@ int snf_top_logits(const void* x, int dtype, int R, int V, int64_t ld, int k, fl
                    void* workspace, int64_t workspace_bytes, snf_stream_t stream);
 int64_t snf_top_distill_workspace_bytes(int R, int V, int dtype);
 int snf_top_distill_fwd(const void* z, int dtype, int R, int V, int64_t ld, const void* ids, int ids_wide, const void* top, int top_dtype,
-                        const float* rest, int K, float temperature, float weight, float* rows, float* counted, float* stats, float* p,
+                        const float* rest, int K, float temperature, float weight, float* rows, float* counted, float* stats, float* diff,
                         int mean, float* loss, float* divisor, void* workspace, int64_t workspace_bytes, snf_stream_t stream);
 int snf_top_distill_bwd(const void* z, int dtype, int R, int V, int64_t ld, const void* ids, int ids_wide, int K, float temperature,
                         float weight, const float* g, int g_per_row, const float* divisor, const float* counted, const float* stats,
-                        const float* p, void* dz, snf_stream_t stream);
+                        const float* diff, void* dz, snf_stream_t stream);
 
 /* ---- microscaled 4-bit floats: the encoder's dense layers with both operands in 4 bits (the reference computes them in fp32:
  *      modeling/image_encoder.py:164-235).

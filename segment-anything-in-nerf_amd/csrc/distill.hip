@@ -581,16 +581,18 @@ __global__ __launch_bounds__(THREADS) void k_top_select(const T* __restrict__ x,
 // other places.  p = softmax over (t / T [, r]), q = softmax(z / T), q_rest = the sum of q over the places that ids does not name:
 //     loss = T^2 [ sum_k p_k (log p_k - log q_{id_k}) + p_rest (log p_rest - log q_rest) ]
 //     dloss / dz_v = T [ q_v - sum_{k: id_k = v} p_k - (v not named) p_rest q_v / q_rest ]
-// Where the list holds little of the mass, p_rest and q_rest are both close to 1, and a difference of their logarithms, or of 1 and their
-// quotient, has none of their digits left.  So with r the loss is taken as
-//     T^2 sum over the entries and the rest of p (log p - log q) + q - p      (- the q of places that are named once more: they count once)
-// -- the additions cancel over all classes, every term is at least 0, and an error of the logarithms counts by p - q alone (td_divergence)
-// --, and what belongs to the rest comes from P and Q, the named places' mass over the rest's on either side, sums that are taken apart:
-//     x = (Q - P) / (1 + P),     log p_rest - log q_rest = log1p(x),     q_v - p_rest q_v / q_rest = -x q_v.
+// Both are differences of numbers that are mostly alike once a student follows its teacher, and where the list holds little of the mass, or
+// one place nearly all of it, also before: sums of p (log p - log q), 1 - p_rest / q_rest and q - p then have no digits left.  So the sums
+// over the named and the other places are taken apart, and
+//   the loss is T^2 sum over the entries and the rest of p (log p - log q) + q - p      (- the q of places that are named once more: they
+//     count once): the additions cancel over all classes, every term is at least 0, an error of the logarithms counts by p - q alone;
+//   with r, P and Q the named places' mass over the rest's on either side and x = (Q - P) / (1 + P):
+//     log p_rest - log q_rest = log1p(x),     q_v - p_rest q_v / q_rest = -x q_v;
+//   at a named place that holds more than half of both masses, q - p is the other places' p less their q.
 // 100000 places, k = 8, T = 4, rows whose divergence is 7e-4: the loss is off by 2e-6 of itself, the other places' gradient by 4e-7 (by
 // 4.5e-3 and 8e-5 as the plain sum of p (log p - log q) and as 1 - p_rest / q_rest).
-// What the backward pass needs of a row (32 + 4 K bytes): its reference m_r, the factor f with dz_v = gs f exp((z_v - m_r) / T) for all
-// places that are not named, the row's maximum m, 1 / sum exp((z - m) / T), and p.
+// What the backward pass needs of a row (12 + 4 K bytes): the reference m_r and the factor f with dz_v = gs f exp((z_v - m_r) / T) for all
+// places that are not named, and q - p of the named ones.
 __device__ __forceinline__ float td_load(const void* p, int dtype, int64_t i) {
     if (dtype == SNF_F32) return reinterpret_cast<const float*>(p)[i];
     if (dtype == SNF_BF16) return (float)reinterpret_cast<const __bf16*>(p)[i];
@@ -609,8 +611,8 @@ struct TdTeacher {
 struct TdSaved {
     float* rows;     // [R] loss of a row, times weight T^2; 0 where there is no target
     float* counted;  // [R] 1 or 0
-    float4* stats;   // [R] m_r, f, m, 1 / sum
-    float* p;        // [R, K]
+    float2* stats;   // [R] m_r, f
+    float* diff;     // [R, K] q - p of a named place at the first entry that names it, 0 at others
 };
 
 // p (log p - log q) + q - p with d = log p - log q, at least 0; near d = 0, where the three cancel, p (d^2 / 2 - d^3 / 6 + ...), whose first
@@ -629,17 +631,20 @@ __device__ __forceinline__ float td_divergence(float p, float q, float d) {
     return p * (d * d * c);
 }
 
-// One wave: the row's teacher side and its loss, from the student's maximum and sum (over the places that are not named where REST).
-template <typename T, bool REST>
+// One wave: the row's teacher side and its loss, from the student's maximum and sum over the places that are not named.
+template <typename T>
 __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V, int64_t row, const TdTeacher& t, float temperature,
                                               float scale, float m_r, float s_r, const TdSaved& out) {
     constexpr int Q = TD_MAX_K / WAVE;
     const int lane = lane_id();
     const float c = TD_LOG2E / temperature;
-    int64_t id[Q];
+    const bool with_rest = t.rest != nullptr;
+    // (the rest is a logarithm of what has been divided by T; without it the difference is taken first)
+    const float before = with_rest ? temperature : 1.f, after = with_rest ? 1.f : temperature;
+    int id[Q];
     float tv[Q], zv[Q];
     bool bad = false, any = false;
-    float tm = TD_NINF;
+    float tm = TD_NINF, nm = TD_NINF;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
         const int k = q * WAVE + lane;
@@ -649,11 +654,11 @@ __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V,
             const int64_t i = td_id(t.ids, t.ids_wide, row * t.K + k);
             bad |= i >= V;
             if (i >= 0 && i < V) {
-                id[q] = i;
+                id[q] = (int)i;
                 any = true;
                 zv[q] = (float)zrow[i];
-                const float l = td_load(t.logits, t.dtype, row * t.K + k);
-                tv[q] = REST ? l / temperature : l;
+                nm = td_max(nm, zv[q]);
+                tv[q] = td_load(t.logits, t.dtype, row * t.K + k) / before;
                 tm = td_max(tm, tv[q]);
             }
         }
@@ -661,100 +666,123 @@ __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V,
     bad = __any(bad);
     any = __any(any) || bad;
     tm = td_reduce_wave<TdMaxOp>(tm);
-    const float r = REST ? t.rest[row] : TD_NINF;
-    if (REST) tm = td_max(tm, r);
+    const float r = with_rest ? t.rest[row] : TD_NINF;
+    if (with_rest) tm = td_max(tm, r);
     if (!any || (tm == TD_NINF && !bad)) {  // no target: no entry, or a teacher without any mass
         if (lane == 0) {
             out.rows[row] = 0.f;
             out.counted[row] = 0.f;
-            out.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+            out.stats[row] = make_float2(0.f, 0.f);
         }
-        for (int k = lane; k < t.K; k += WAVE) out.p[row * t.K + k] = 0.f;
+        for (int k = lane; k < t.K; k += WAVE) out.diff[row * t.K + k] = 0.f;
         return;
     }
-    // teacher
+    // teacher: exponentials, their sum
     float pe[Q], ps = 0.f;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-        tv[q] = REST ? tv[q] - tm : (tv[q] - tm) / temperature;
+        tv[q] = (tv[q] - tm) / after;
         pe[q] = id[q] >= 0 ? expf(tv[q]) : 0.f;
         ps += pe[q];
     }
     const float pn = td_reduce_wave<TdSumOp>(ps);
-    const float re = REST ? expf(r - tm) : 0.f;
+    const float re = with_rest ? expf(r - tm) : 0.f;
     ps = pn + re;
-    const float log_ps = logf(ps);
-    // student
-    float m = m_r, s = s_r, sn = 0.f, rest_scale = 1.f, loss = 0.f, en[Q];
-    if (REST) {  // the named places, each once
-        float nm = TD_NINF;
+    // student: the named places, each once (and the mass of those that are named again)
+    nm = td_reduce_wave<TdMaxOp>(nm);
+    const float m = td_max(m_r, nm);
+    float en[Q], sn = 0.f, again = 0.f;
+    bool first[Q], twice = false;
 #pragma unroll
-        for (int q = 0; q < Q; ++q) nm = td_max(nm, zv[q]);
-        nm = td_reduce_wave<TdMaxOp>(nm);
-        m = td_max(m_r, nm);
-        float again = 0.f;
+    for (int q = 0; q < Q; ++q) {
+        en[q] = 0.f;
+        first[q] = id[q] >= 0;
+        if (q * WAVE >= t.K) continue;
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            en[q] = 0.f;
-            if (q * WAVE >= t.K) break;
-            bool first = id[q] >= 0;
-#pragma unroll
-            for (int q2 = 0; q2 <= q; ++q2)
-                for (int l = 0; l < (q2 < q ? WAVE : WAVE - 1); ++l) {
-                    if (q2 * WAVE + l >= t.K) break;
-                    const int other = __builtin_amdgcn_readlane((int)id[q2], l);
-                    if (q2 * WAVE + l < q * WAVE + lane && other == (int)id[q]) first = false;
-                }
-            if (id[q] >= 0) {
-                en[q] = td_term(zv[q], m, c);
-                if (first) sn += en[q];
-                else again += en[q];
+        for (int q2 = 0; q2 <= q; ++q2)
+            for (int l = 0; l < (q2 < q ? WAVE : WAVE - 1); ++l) {
+                if (q2 * WAVE + l >= t.K) break;
+                const int other = __builtin_amdgcn_readlane(id[q2], l);
+                if (q2 * WAVE + l < q * WAVE + lane && other == id[q]) first[q] = false;
             }
+        if (id[q] >= 0) {
+            en[q] = td_term(zv[q], m, c);
+            if (first[q]) sn += en[q];
+            else again += en[q];
+            twice |= !first[q];
         }
-        sn = td_reduce_wave<TdSumOp>(sn);
-        rest_scale = td_term(m_r, m, c);
-        s = sn + s_r * rest_scale;
-        loss -= again / s;
     }
-    const float log_s = logf(s);
+    sn = td_reduce_wave<TdSumOp>(sn);
+    const float rest_scale = td_term(m_r, m, c), su = s_r * rest_scale, s = sn + su;
+    // loss
+    const float log_ps = logf(ps), log_s = logf(s);
+    float loss = -again / s;
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        if (id[q] >= 0) loss += td_divergence(pe[q] / ps, en[q] / s, (tv[q] - log_ps) - ((zv[q] - m) / temperature - log_s));
+    loss = td_reduce_wave<TdSumOp>(loss);
+    const float pr = re / ps, P = pn / re, x = (sn / su - P) / (1.f + P);  // (x is not finite where one of the rests has no mass)
+    const bool near = fabsf(x) <= 0.5f;
+    const float d = near ? log1pf(x) : (r - tm - log_ps) - ((m_r - m) / temperature + logf(s_r) - log_s);
+    loss += td_divergence(pr, su / s, d);
+    // gradient
+    float ref = m_r, f = near ? -x * rest_scale / s : rest_scale / s - (pr == 0.f ? 0.f : pr / s_r);
+    if (m_r == TD_NINF) { ref = 0.f; f = 0.f; }  // every place is named, or what is not is -inf
+    float pv[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) pv[q] = pe[q];
+    if (__any(twice)) {
+#pragma unroll
+        for (int q2 = 0; q2 < Q; ++q2)
+            for (int l = 0; l < WAVE; ++l) {
+                if (q2 * WAVE + l >= t.K) break;
+                const int other = __builtin_amdgcn_readlane(id[q2], l);
+                const float mass = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pe[q2]), l));
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+                    if (other == id[q] && (q2 != q || l != lane)) pv[q] += mass;
+            }
+    }
+    int heavy = -1;  // the named place with more than half of both masses, if there is one
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        if (first[q] && en[q] > 0.5f * s && pv[q] > 0.5f * ps) heavy = id[q];
+    const uint64_t found = __ballot(heavy >= 0);
+    float heavy_diff = 0.f;
+    if (found) {
+        heavy = __builtin_amdgcn_readlane(heavy, __builtin_ctzll(found));
+        float po = 0.f, qo = 0.f;
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            if (id[q] != heavy) {
+                po += pe[q];
+                if (first[q]) qo += en[q];
+            }
+        po = td_reduce_wave<TdSumOp>(po) + re;
+        qo = td_reduce_wave<TdSumOp>(qo) + su;
+        heavy_diff = po / ps - qo / s;
+    }
+    if (bad) loss = f = __uint_as_float(0x7FC00000u);  // an id past the end
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
         const int k = q * WAVE + lane;
-        if (q * WAVE >= t.K) break;
-        const float p = pe[q] / ps;
-        if (k < t.K) out.p[row * t.K + k] = p;
-        if (id[q] < 0) continue;
-        const float d = (tv[q] - log_ps) - ((zv[q] - m) / temperature - log_s);
-        if (REST) loss += td_divergence(p, en[q] / s, d);
-        else if (p > 0.f || p != p) loss += p * d;
+        const float diff = !first[q] ? 0.f : id[q] == heavy ? heavy_diff : en[q] / s - pv[q] / ps;
+        if (k < t.K) out.diff[row * t.K + k] = bad ? f : diff;
     }
-    loss = td_reduce_wave<TdSumOp>(loss);
-    float f = 1.f / s, ref = m;
-    if (REST) {
-        const float pr = re / ps, su = s_r * rest_scale;
-        const float P = pn / re, x = (sn / su - P) / (1.f + P);  // (not finite where one of the rests has no mass)
-        const bool near = fabsf(x) <= 0.5f;
-        const float d = near ? log1pf(x) : (r - tm - log_ps) - ((m_r - m) / temperature + logf(s_r) - log_s);
-        loss += td_divergence(pr, su / s, d);
-        ref = m_r;
-        f = near ? -x * rest_scale / s : rest_scale / s - (pr > 0.f || pr != pr ? pr / s_r : 0.f);
-        if (m_r == TD_NINF) { ref = 0.f; f = 0.f; }  // every place is named, or what is not is -inf
-    }
-    if (bad) loss = f = __uint_as_float(0x7FC00000u);  // an id past the end
     if (lane == 0) {
         out.rows[row] = loss * scale;
         out.counted[row] = 1.f;
-        out.stats[row] = make_float4(ref, f, m, bad ? f : 1.f / s);
+        out.stats[row] = make_float2(ref, f);
     }
 }
 
-template <typename T, bool REST, int THREADS, int NV>
+template <typename T, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS) void k_top_distill_rows(const T* __restrict__ z, int V, int64_t ld, TdTeacher t, float temperature,
                                                               float scale, int parts, int part_len, TdSaved out,
                                                               float2* __restrict__ part_ms) {
     using Part = TdPart<T, THREADS, NV>;
     constexpr int WORDS = (THREADS * NV * Part::E + 31) / 32;
-    __shared__ uint32_t s_named[REST ? WORDS : 1];
+    __shared__ uint32_t s_named[WORDS];
     __shared__ float s_red[THREADS / WAVE];
     const int64_t row = blockIdx.x / (unsigned)parts;
     const int part = (int)(blockIdx.x % (unsigned)parts);
@@ -762,26 +790,25 @@ __global__ __launch_bounds__(THREADS) void k_top_distill_rows(const T* __restric
     const T* zrow = z + row * ld;
     // (the ids are asked for before the row: loads come back in order)
     int64_t first_id = -1;
-    if (REST && (int)threadIdx.x < t.K) first_id = td_id(t.ids, t.ids_wide, row * t.K + threadIdx.x);
+    if ((int)threadIdx.x < t.K) first_id = td_id(t.ids, t.ids_wide, row * t.K + threadIdx.x);
     Part reg;
     reg.load(zrow + p0, len);
-    if (REST) {  // the named places become -inf: one bit per place of the part, in the order of the registers
-        for (int i = threadIdx.x; i < WORDS; i += THREADS) s_named[i] = 0;
-        __syncthreads();
-        for (int k = threadIdx.x; k < t.K; k += THREADS) {
-            const int64_t i = (k < THREADS ? first_id : td_id(t.ids, t.ids_wide, row * t.K + k)) - p0;
-            if (i >= 0 && i < len) atomicOr(&s_named[(i + reg.shift) >> 5], 1u << ((i + reg.shift) & 31));
-        }
-        __syncthreads();
+    // the named places become -inf: one bit per place of the part, in the order of the registers
+    for (int i = threadIdx.x; i < WORDS; i += THREADS) s_named[i] = 0;
+    __syncthreads();
+    for (int k = threadIdx.x; k < t.K; k += THREADS) {
+        const int64_t i = (k < THREADS ? first_id : td_id(t.ids, t.ids_wide, row * t.K + k)) - p0;
+        if (i >= 0 && i < len) atomicOr(&s_named[(i + reg.shift) >> 5], 1u << ((i + reg.shift) & 31));
+    }
+    __syncthreads();
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int b = (j * THREADS + (int)threadIdx.x) * Part::E;
-            const uint32_t bits = s_named[b >> 5] >> (b & 31) & ((1u << Part::E) - 1u);
-            if (bits)
+    for (int j = 0; j < NV; ++j) {
+        const int b = (j * THREADS + (int)threadIdx.x) * Part::E;
+        const uint32_t bits = s_named[b >> 5] >> (b & 31) & ((1u << Part::E) - 1u);
+        if (bits)
 #pragma unroll
-                for (int e = 0; e < Part::E; ++e)
-                    if (bits >> e & 1u) td_clear<T>(reg.r[j], e);
-        }
+            for (int e = 0; e < Part::E; ++e)
+                if (bits >> e & 1u) td_clear<T>(reg.r[j], e);
     }
     const float c = TD_LOG2E / temperature;
     float m = TD_NINF, s = 0.f;
@@ -792,12 +819,12 @@ __global__ __launch_bounds__(THREADS) void k_top_distill_rows(const T* __restric
     if (parts > 1) {
         if (threadIdx.x == 0) part_ms[row * parts + part] = make_float2(m, s);
     } else if (threadIdx.x < WAVE) {
-        td_finish_row<T, REST>(zrow, V, row, t, temperature, scale, m, s, out);
+        td_finish_row<T>(zrow, V, row, t, temperature, scale, m, s, out);
     }
 }
 
 // rows in parts: the parts' maxima and sums joined, then the row as above; one wave per row
-template <typename T, bool REST>
+template <typename T>
 __global__ __launch_bounds__(64) void k_top_distill_join(const T* __restrict__ z, int V, int64_t ld, TdTeacher t, float temperature,
                                                          float scale, int parts, TdSaved out, const float2* __restrict__ part_ms) {
     const int64_t row = blockIdx.x;
@@ -810,7 +837,7 @@ __global__ __launch_bounds__(64) void k_top_distill_join(const T* __restrict__ z
         s += ms.y * td_term(ms.x, m, c);
     }
     s = td_reduce_wave<TdSumOp>(s);
-    td_finish_row<T, REST>(z + row * ld, V, row, t, temperature, scale, m, s, out);
+    td_finish_row<T>(z + row * ld, V, row, t, temperature, scale, m, s, out);
 }
 
 // the loss, and what the rows' gradients are divided by; one workgroup, sums in a fixed order
@@ -839,23 +866,23 @@ template <typename T, bool PACKED>
 __global__ __launch_bounds__(256) void k_top_distill_bwd(const T* __restrict__ z, int V, int64_t ld, const void* __restrict__ ids,
                                                          int ids_wide, int K, float temperature, float scale, int chunks,
                                                          const float* __restrict__ g, int g_per_row, const float* __restrict__ divisor,
-                                                         const float* __restrict__ counted, const float4* __restrict__ stats,
-                                                         const float* __restrict__ p, T* __restrict__ dz) {
+                                                         const float* __restrict__ counted, const float2* __restrict__ stats,
+                                                         const float* __restrict__ diff, T* __restrict__ dz) {
     constexpr int E = 16 / (int)sizeof(T);
     __shared__ uint32_t s_named[TD_CHUNK / 32 + 1];
     __shared__ int s_id[TD_MAX_K];
-    __shared__ float s_p[TD_MAX_K];
+    __shared__ float s_diff[TD_MAX_K];
     constexpr int KEEP = 4;
     const int64_t row = blockIdx.x / (unsigned)chunks;
     const int p0 = (int)(blockIdx.x % (unsigned)chunks) * TD_CHUNK, len = min(TD_CHUNK, V - p0);
     const T* zp = z + row * ld + p0;
     T* dp = dz + row * V + p0;
-    // what does not depend on anything is asked for first: the row's scalars, a thread's id and p, its first granules
+    // what does not depend on anything is asked for first: the row's scalars, a thread's id and its q - p, its first granules
     int64_t first_id = -1;
-    float first_p = 0.f;
+    float first_diff = 0.f;
     if ((int)threadIdx.x < K) {
         first_id = td_id(ids, ids_wide, row * K + threadIdx.x);
-        first_p = p[row * K + threadIdx.x];
+        first_diff = diff[row * K + threadIdx.x];
     }
     const int shift = PACKED ? (int)((reinterpret_cast<uintptr_t>(zp) & 15) / sizeof(T)) : 0;
     const int granules = (shift + len + E - 1) / E;
@@ -868,7 +895,7 @@ __global__ __launch_bounds__(256) void k_top_distill_bwd(const T* __restrict__ z
     const bool live = counted[row] != 0.f;
     const float gs = g[g_per_row ? row : 0] * scale / (divisor ? divisor[0] : 1.f);
     const float c = TD_LOG2E / temperature;
-    const float4 st = stats[row];
+    const float2 st = stats[row];
     const float f = gs * st.y;
     if (live) {
         for (int i = threadIdx.x; i <= (shift + len) / 32; i += blockDim.x) s_named[i] = 0;
@@ -877,7 +904,7 @@ __global__ __launch_bounds__(256) void k_top_distill_bwd(const T* __restrict__ z
             const int64_t i = (k < (int)blockDim.x ? first_id : td_id(ids, ids_wide, row * K + k)) - p0;
             const bool here = i >= 0 && i < len;
             s_id[k] = here ? (int)i : -1;
-            s_p[k] = k < (int)blockDim.x ? first_p : p[row * K + k];
+            s_diff[k] = k < (int)blockDim.x ? first_diff : diff[row * K + k];
             if (here) atomicOr(&s_named[(i + shift) >> 5], 1u << ((i + shift) & 31));
         }
         __syncthreads();
@@ -889,9 +916,9 @@ __global__ __launch_bounds__(256) void k_top_distill_bwd(const T* __restrict__ z
             for (int o = 0; o < K; ++o)
                 if (s_id[o] == i) {
                     first &= o >= k;
-                    sum += s_p[o];
+                    sum += s_diff[o];  // (not 0 once at most)
                 }
-            if (first) dp[i] = (T)(gs * (td_exp2(((float)zp[i] - st.z) * c) * st.w - sum));
+            if (first) dp[i] = (T)(gs * sum);
         }
     }
     if constexpr (PACKED) {
@@ -995,7 +1022,7 @@ static int td_top_t(const T* x, int R, int V, int64_t ld, int k, float temperatu
     return SNF_OK;
 }
 
-template <typename T, bool REST>
+template <typename T>
 static int td_fwd_t(const T* z, int R, int V, int64_t ld, const TdTeacher& t, float temperature, float weight, const TdSaved& out, void* ws,
                     hipStream_t st) {
     const TdPlan pl = td_rows_plan(R, V, 16 / (int)sizeof(T));
@@ -1004,14 +1031,14 @@ static int td_fwd_t(const T* z, int R, int V, int64_t ld, const TdTeacher& t, fl
     const dim3 grid((unsigned)((int64_t)R * pl.parts));
 #define TD_GO(S_)                                                                                                                     \
     case S_:                                                                                                                          \
-        k_top_distill_rows<T, REST, TD_SHAPES[S_].threads, TD_SHAPES[S_].nv><<<grid, dim3(TD_SHAPES[S_].threads), 0, st>>>(           \
+        k_top_distill_rows<T, TD_SHAPES[S_].threads, TD_SHAPES[S_].nv><<<grid, dim3(TD_SHAPES[S_].threads), 0, st>>>(           \
             z, V, ld, t, temperature, scale, pl.parts, pl.part_len, out, (float2*)ws);                                                \
         break;
     switch (pl.shape) { TD_GO(0) TD_GO(1) TD_GO(2) }
 #undef TD_GO
     SNF_LAUNCH_CHECK("snf_top_distill_fwd");
     if (pl.parts > 1) {
-        k_top_distill_join<T, REST><<<dim3(R), dim3(64), 0, st>>>(z, V, ld, t, temperature, scale, pl.parts, out, (const float2*)ws);
+        k_top_distill_join<T><<<dim3(R), dim3(64), 0, st>>>(z, V, ld, t, temperature, scale, pl.parts, out, (const float2*)ws);
         SNF_LAUNCH_CHECK("snf_top_distill_fwd (join)");
     }
     return SNF_OK;
@@ -1025,8 +1052,8 @@ static int td_mean(const float* rows, const float* counted, int R, int mean, flo
 
 template <typename T>
 static int td_bwd_t(const T* z, int R, int V, int64_t ld, const void* ids, int ids_wide, int K, float temperature, float weight,
-                    const float* g, int g_per_row, const float* divisor, const float* counted, const float4* stats, const float* p, T* dz,
-                    hipStream_t st) {
+                    const float* g, int g_per_row, const float* divisor, const float* counted, const float2* stats, const float* diff,
+                    T* dz, hipStream_t st) {
     const int chunks = ceil_div(V, TD_CHUNK);
     SNF_REQUIRE((int64_t)R * chunks * 256 < ((int64_t)1 << 32), "snf_top_distill_bwd: %d rows of %d are too many for one launch", R, V);
     const dim3 grid((unsigned)((int64_t)R * chunks)), block(V <= 1024 ? 64 : 256);
@@ -1034,10 +1061,10 @@ static int td_bwd_t(const T* z, int R, int V, int64_t ld, const void* ids, int i
     const bool packed = (R == 1 || zb == db) && (reinterpret_cast<uintptr_t>(z) & 15) == (reinterpret_cast<uintptr_t>(dz) & 15);
     if (packed)
         k_top_distill_bwd<T, true><<<grid, block, 0, st>>>(z, V, ld, ids, ids_wide, K, temperature, weight * temperature, chunks, g, g_per_row,
-                                                           divisor, counted, stats, p, dz);
+                                                           divisor, counted, stats, diff, dz);
     else
         k_top_distill_bwd<T, false><<<grid, block, 0, st>>>(z, V, ld, ids, ids_wide, K, temperature, weight * temperature, chunks, g,
-                                                            g_per_row, divisor, counted, stats, p, dz);
+                                                            g_per_row, divisor, counted, stats, diff, dz);
     SNF_LAUNCH_CHECK("snf_top_distill_bwd");
     return SNF_OK;
 }
@@ -1078,7 +1105,7 @@ int64_t snf_top_distill_workspace_bytes(int R, int V, int dtype) {
 }
 
 int snf_top_distill_fwd(const void* z, int dtype, int R, int V, int64_t ld, const void* ids, int ids_wide, const void* top, int top_dtype,
-                        const float* rest, int K, float temperature, float weight, float* rows, float* counted, float* stats, float* p,
+                        const float* rest, int K, float temperature, float weight, float* rows, float* counted, float* stats, float* diff,
                         int mean, float* loss, float* divisor, void* workspace, int64_t workspace_bytes, snf_stream_t stream) {
     SNF_REQUIRE(R >= 0 && V >= 1 && V <= SNF_TOP_MAX_V, "snf_top_distill_fwd: bad sizes R=%d V=%d", R, V);
     SNF_REQUIRE(K >= 1 && K <= snf::TD_MAX_K, "snf_top_distill_fwd: K=%d is not in 1 .. %d", K, snf::TD_MAX_K);
@@ -1087,15 +1114,14 @@ int snf_top_distill_fwd(const void* z, int dtype, int R, int V, int64_t ld, cons
     SNF_REQUIRE(!loss || divisor, "snf_top_distill_fwd: null pointer");
     hipStream_t st = (hipStream_t)stream;
     if (R == 0) return loss ? snf::td_mean(rows, counted, R, mean, loss, divisor, st) : SNF_OK;
-    SNF_REQUIRE(z && ids && top && rows && counted && stats && p, "snf_top_distill_fwd: null pointer");
-    SNF_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0, "snf_top_distill_fwd: stats is not aligned to 16 bytes");
+    SNF_REQUIRE(z && ids && top && rows && counted && stats && diff, "snf_top_distill_fwd: null pointer");
+    SNF_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "snf_top_distill_fwd: stats is not aligned to 8 bytes");
     SNF_REQUIRE(ld >= V || R == 1, "snf_top_distill_fwd: rows of %d values overlap at stride %lld", V, (long long)ld);
     SNF_REQUIRE(workspace_bytes >= snf_top_distill_workspace_bytes(R, V, dtype) && (workspace_bytes == 0 || workspace),
                 "snf_top_distill_fwd: workspace of %lld bytes is too small", (long long)workspace_bytes);
     const snf::TdTeacher t{ids, top, rest, ids_wide, top_dtype, K};
-    const snf::TdSaved out{rows, counted, (float4*)stats, p};
-#define TD_T(T_) (rest ? snf::td_fwd_t<T_, true>((const T_*)z, R, V, ld, t, temperature, weight, out, workspace, st)                  \
-                       : snf::td_fwd_t<T_, false>((const T_*)z, R, V, ld, t, temperature, weight, out, workspace, st))
+    const snf::TdSaved out{rows, counted, (float2*)stats, diff};
+#define TD_T(T_) snf::td_fwd_t<T_>((const T_*)z, R, V, ld, t, temperature, weight, out, workspace, st)
     const int rc = dtype == SNF_F32 ? TD_T(float) : dtype == SNF_BF16 ? TD_T(__bf16) : TD_T(_Float16);
 #undef TD_T
     return rc != SNF_OK || !loss ? rc : snf::td_mean(rows, counted, R, mean, loss, divisor, st);
@@ -1103,18 +1129,18 @@ int snf_top_distill_fwd(const void* z, int dtype, int R, int V, int64_t ld, cons
 
 int snf_top_distill_bwd(const void* z, int dtype, int R, int V, int64_t ld, const void* ids, int ids_wide, int K, float temperature,
                         float weight, const float* g, int g_per_row, const float* divisor, const float* counted, const float* stats,
-                        const float* p, void* dz, snf_stream_t stream) {
+                        const float* diff, void* dz, snf_stream_t stream) {
     SNF_REQUIRE(R >= 0 && V >= 1 && V <= SNF_TOP_MAX_V, "snf_top_distill_bwd: bad sizes R=%d V=%d", R, V);
     SNF_REQUIRE(K >= 1 && K <= snf::TD_MAX_K, "snf_top_distill_bwd: K=%d is not in 1 .. %d", K, snf::TD_MAX_K);
     SNF_REQUIRE(temperature >= FLT_MIN && temperature < INFINITY, "snf_top_distill_bwd: temperature %g", (double)temperature);
     SNF_REQUIRE(dtype >= SNF_F32 && dtype <= SNF_F16, "snf_top_distill_bwd: unknown dtype %d", dtype);
     if (R == 0) return SNF_OK;
-    SNF_REQUIRE(z && ids && g && counted && stats && p && dz, "snf_top_distill_bwd: null pointer");
-    SNF_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0, "snf_top_distill_bwd: stats is not aligned to 16 bytes");
+    SNF_REQUIRE(z && ids && g && counted && stats && diff && dz, "snf_top_distill_bwd: null pointer");
+    SNF_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "snf_top_distill_bwd: stats is not aligned to 8 bytes");
     SNF_REQUIRE(ld >= V || R == 1, "snf_top_distill_bwd: rows of %d values overlap at stride %lld", V, (long long)ld);
     hipStream_t st = (hipStream_t)stream;
-    const float4* s4 = (const float4*)stats;
-#define TD_T(T_) snf::td_bwd_t<T_>((const T_*)z, R, V, ld, ids, ids_wide, K, temperature, weight, g, g_per_row, divisor, counted, s4, p,   \
+    const float2* s2 = (const float2*)stats;
+#define TD_T(T_) snf::td_bwd_t<T_>((const T_*)z, R, V, ld, ids, ids_wide, K, temperature, weight, g, g_per_row, divisor, counted, s2, diff, \
                                    (T_*)dz, st)
     switch (dtype) {
         case SNF_F32: return TD_T(float);

@@ -67,7 +67,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
 
 
 class _TopDistill(torch.autograd.Function):
-    # one buffer of floats: stats [R, 4], p [R, K], counted [R], the divisor, rows [R] (unless they are the result)
+    # one buffer of floats: stats [R, 2], diff [R, K], counted [R], the divisor, rows [R] (unless they are the result)
     @staticmethod
     def forward(ctx, student, ids, logits, rest, temperature: float, weight: float, reduction: str):
         dev = student.device
@@ -78,15 +78,15 @@ class _TopDistill(torch.autograd.Function):
         R = z.shape[0]
         code = DTYPE_CODE[z.dtype]
         per_row = reduction == "none"
-        saved = torch.empty((R * (6 + K) + 1,), device=dev, dtype=torch.float32)
+        saved = torch.empty((R * (4 + K) + 1,), device=dev, dtype=torch.float32)
         at = saved.data_ptr()
-        counted, divisor, rows = at + 4 * R * (4 + K), at + 4 * R * (5 + K), at + 4 * R * (5 + K) + 4
+        counted, divisor, rows = at + 4 * R * (2 + K), at + 4 * R * (3 + K), at + 4 * R * (3 + K) + 4
         loss = torch.empty(student.shape[:-1] if per_row else (), device=dev, dtype=torch.float32)
         if R or not per_row:
             nbytes = int(_L().snf_top_distill_workspace_bytes(R, V, code))
             ws = _workspace(nbytes, dev)
             _launch("snf_top_distill_fwd", _p(z), code, R, V, ld, _p(ids), int(ids.dtype == torch.int64), _p(logits),
-                    DTYPE_CODE[logits.dtype], _p(rest), K, temperature, weight, _p(loss) if per_row else rows, counted, at, at + 16 * R,
+                    DTYPE_CODE[logits.dtype], _p(rest), K, temperature, weight, _p(loss) if per_row else rows, counted, at, at + 8 * R,
                     int(reduction == "mean"), None if per_row else _p(loss), divisor, _p(ws), nbytes, _stream_on(student.get_device()),
                     units=float(R * V * z.element_size()))
         ctx.args = (student.shape, R, V, ld, K, temperature, weight, per_row)
@@ -110,9 +110,9 @@ class _TopDistill(torch.autograd.Function):
             if g.dtype != torch.float32 or not g.is_contiguous():
                 g = g.to(torch.float32).contiguous()
             at = saved.data_ptr()
-            counted, divisor = at + 4 * R * (4 + K), at + 4 * R * (5 + K)
+            counted, divisor = at + 4 * R * (2 + K), at + 4 * R * (3 + K)
             _launch("snf_top_distill_bwd", _p(z), DTYPE_CODE[z.dtype], R, V, ld, _p(ids), int(ids.dtype == torch.int64), K, temperature,
-                    weight, _p(g), int(per_row), None if per_row else divisor, counted, at, at + 16 * R, _p(dz), _stream_on(z.get_device()),
+                    weight, _p(g), int(per_row), None if per_row else divisor, counted, at, at + 8 * R, _p(dz), _stream_on(z.get_device()),
                     units=float(2 * R * V * z.element_size()))
         return dz, None, None, None, None, None, None
 

@@ -1,6 +1,7 @@
 """GPU tests of a teacher's top logits and the distillation loss that reads them (csrc/distill.hip), against their definition in 64 bits."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -423,15 +424,33 @@ def test_distill_repeats_streams_and_graphs(R, V):
         assert all(torch.equal(a, b) for a, b in zip(t2, tops[i]))
 
 
-def classes64(z, ids, top, rest, T):
-    """Of rows whose ids are all entries, in float64: the teacher's mass per place [R, V] and of the rest [R], q [R, V], which are named."""
+def classes80(z, ids, top, rest, T):
+    """Of rows whose ids are all entries: the teacher's mass per place [R, V] and of the rest [R], q [R, V], which are named, the rows' loss
+    and its gradient.  Computed in 80 bits: at 1e-11 of a probability close to 1, 64 have four digits."""
+    f80 = lambda t: np.asarray(t.double().numpy(), dtype=np.longdouble)  # noqa: E731
     R, V = z.shape
-    a = top.double() / T
-    lse = torch.logsumexp(a if rest is None else torch.cat([a, rest.double()[:, None]], 1), 1, keepdim=True)
-    p = torch.zeros((R, V), dtype=torch.float64).scatter_add_(1, ids.long(), torch.exp(a - lse))
-    pr = torch.exp(rest.double() - lse[:, 0]) if rest is not None else torch.zeros(R, dtype=torch.float64)
-    named = torch.zeros((R, V), dtype=torch.bool).scatter_(1, ids.long(), True)
-    return p, pr, torch.softmax(z.double() / T, 1), named
+    row, i = np.arange(R)[:, None], ids.long().numpy()
+    a = f80(top) / np.longdouble(T)
+    if rest is not None:
+        a = np.concatenate([a, f80(rest)[:, None]], 1)
+    am = a.max(1, keepdims=True)
+    lp = a - am - np.log(np.exp(a - am).sum(1, keepdims=True))
+    u = f80(z) / np.longdouble(T)
+    um = u.max(1, keepdims=True)
+    logq = u - um - np.log(np.exp(u - um).sum(1, keepdims=True))
+    q = np.exp(logq)
+    K = i.shape[1]
+    p, named = np.zeros((R, V), np.longdouble), np.zeros((R, V), bool)
+    np.add.at(p, (row, i), np.exp(lp[:, :K]))
+    named[row, i] = True
+    loss = (np.exp(lp[:, :K]) * (lp[:, :K] - logq[row, i])).sum(1)
+    dz, pr = q - p, np.zeros(R, np.longdouble)
+    if rest is not None:
+        pr, other = np.exp(lp[:, -1]), (q * ~named).sum(1)
+        loss += pr * (lp[:, -1] - np.log(other))
+        dz -= np.where(named, 0, q) * (pr / other)[:, None]
+    f64 = lambda a: torch.from_numpy(a.astype(np.float64))  # noqa: E731
+    return f64(p), f64(pr), f64(q), torch.from_numpy(named), f64(loss * np.longdouble(T) ** 2), f64(dz * np.longdouble(T))
 
 
 def check_digits(z, ids, top, rest, T):
@@ -440,8 +459,7 @@ def check_digits(z, ids, top, rest, T):
     logits over T, and by what the sums are off: 64 places a lane in turn, a tree, some thousand parts joined by lanes, exponentials of
     exponents up to 30 (3 steps each): 160 + 90 steps.  Probabilities in p d + q - p: the same, at most 6 times the term."""
     from samnerf_amd import ops
-    p, pr, q, named = classes64(z, ids, top, rest, T)
-    rows, _ = loss64(z.double(), ids, top.double(), rest.double() if rest is not None else None, T)
+    p, pr, q, named, rows, want = classes80(z, ids, top, rest, T)
     pn, qn = p.sum(1), (q * named).sum(1)
     qr = (q * ~named).sum(1)
     size = (z.double().abs().max(1).values + top.double().abs().max(1).values) / T + (rest.double().abs() if rest is not None else 0)
@@ -457,12 +475,18 @@ def check_digits(z, ids, top, rest, T):
     # 3 steps of its exponent; then the result's own rounding
     fi = torch.finfo(z.dtype)
     share = q / qr.clamp_min(1e-300)[:, None]
-    want = T * (q - (pr[:, None] * share if rest is not None else 0))
     far = 3 * (z.double().max(1, keepdim=True).values - z.double()) / T + 8
     gtol = T * share * U * ((steps * (pn + qn))[:, None] if rest is not None else steps[:, None] * qr[:, None]) + want.abs() * (U * far + fi.eps / 2 * 1.01)
     bad = ((dx.cpu().double() - want).abs() > gtol + fi.smallest_normal * fi.eps) & ~named
     assert not bool(bad.any()), ((dx.cpu().double() - want).abs() / gtol)[bad].max()
-    return dx.cpu().double(), p, q, named, steps
+    return dx.cpu().double(), want, p, pr, q, named, steps
+
+
+def grad_of_sum(z, ids, top, rest, T=1.0):
+    from samnerf_amd import ops
+    x = z.cuda().requires_grad_(True)
+    loss = ops.top_logits_distill_loss(x, ids.cuda(), top.cuda(), rest=rest.cuda() if rest is not None else None, temperature=T, reduction="sum")
+    return torch.autograd.grad(loss, x)[0].cpu().double()
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -473,6 +497,49 @@ def test_distill_short_list_of_a_long_row(k, V, dtype):
     for T in (2.0, 4.0):
         for R in (1, 24):
             check_digits(*make(R, V, k, dtype, V + k + R, empty=0, T=T), T)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("with_rest", [False, True])
+@pytest.mark.parametrize("V,k", [(2, 1), (2, 2), (40, 7), (1003, 16), (9000, 130), (70000, 64)])
+def test_distill_one_place_holds_nearly_all(V, k, with_rest, dtype):
+    """One named place with nearly all of both masses, the last entry of the list or the first: its q - p is the others' p less their q, and
+    the loss is of their size."""
+    for T, gap in ((1.0, 12.0), (0.5, 4.0), (3.0, 45.0)):
+        z, ids, top, rest = make(6, V, k, torch.float32, V + k, empty=0, with_rest=with_rest, T=T)
+        if rest is not None and k == V:
+            continue  # (nothing is left for the rest)
+        up = gap + 2 * T * math.log(V)
+        j = torch.arange(6) % k
+        row = torch.arange(6)
+        top[row, j] += up
+        z[row, ids[row, j].long()] += up
+        z, top = z.to(dtype), top.to(dtype)
+        d, want, p, pr, q, named, steps = check_digits(z, ids, top, rest, T)
+        others = 1 - torch.nn.functional.one_hot(ids[row, j].long(), V)
+        of_others = ((p + q) * others).sum(1) + pr
+        apart = torch.where(others == 0, of_others[:, None].expand(6, V), p + q)
+        fi = torch.finfo(dtype)
+        tol = T * U * steps[:, None] * apart + want.abs() * fi.eps / 2 * 1.01 + fi.smallest_normal * fi.eps
+        bad = ((d - want).abs() > tol) & named
+        assert not bool(bad.any()), ((d - want).abs() / tol)[bad].max()
+
+
+def test_distill_place_named_twice_holds_nearly_all():
+    """Two entries for the heavy place, first and last of the list: their masses add up, the place counts once for the student."""
+    for with_rest in (False, True):
+        z, ids, top, rest = make(4, 300, 6, torch.float32, 9, empty=0, with_rest=with_rest)
+        ids[:, 5] = ids[:, 0]
+        top[:, 0] += 14.0
+        top[:, 5] = top[:, 0] - 1.0
+        z[torch.arange(4), ids[:, 0].long()] += 16.0
+        check_loss(z, ids, top, rest, 1.0)
+        p, pr, q, named, _, want = classes80(z, ids, top, rest, 1.0)
+        d = grad_of_sum(z, ids, top, rest)
+        heavy = torch.nn.functional.one_hot(ids[:, 0].long(), 300).bool()
+        of_others = ((p + q) * ~heavy).sum(1) + pr
+        steps = 250 + 8 * (z.double().abs().max(1).values + top.double().abs().max(1).values + (0 if rest is None else rest.double().abs()))
+        assert bool(((d - want).abs()[heavy] <= U * steps * of_others).all())  # (as check_digits)
 
 
 def test_refusals_at_the_library():
