@@ -696,15 +696,19 @@ __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V,
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
         en[q] = 0.f;
-        first[q] = id[q] >= 0;
+        first[q] = false;
         if (q * WAVE >= t.K) continue;
+        uint64_t named = 0;  // lanes whose place an earlier entry names
 #pragma unroll
         for (int q2 = 0; q2 <= q; ++q2)
-            for (int l = 0; l < (q2 < q ? WAVE : WAVE - 1); ++l) {
-                if (q2 * WAVE + l >= t.K) break;
-                const int other = __builtin_amdgcn_readlane(id[q2], l);
-                if (q2 * WAVE + l < q * WAVE + lane && other == id[q]) first[q] = false;
+            for (int l0 = 0; l0 < WAVE && q2 * WAVE + l0 < t.K; l0 += 8) {
+#pragma unroll
+                for (int l = l0; l < l0 + 8; ++l) {
+                    const uint64_t same = __ballot(id[q] == __builtin_amdgcn_readlane(id[q2], l));
+                    named |= q2 < q ? same : same & (~1ull << l);
+                }
             }
+        first[q] = id[q] >= 0 && !(named >> lane & 1);
         if (id[q] >= 0) {
             en[q] = td_term(zv[q], m, c);
             if (first[q]) sn += en[q];
