@@ -61,8 +61,26 @@ __device__ __forceinline__ float td_value(uint32_t key) {
 }
 __device__ __forceinline__ float td_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // a NaN stays
 __device__ __forceinline__ float td_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-// exp((x - m) / T), c = log2(e) / T; nothing is left of x = -inf, also where the maximum is
+// exp((x - m) / T), c = log2(e) / T; nothing is left of x = -inf, also where the maximum is.  x - m, c and their product are rounded to
+// 32 bits: off by up to 3 |x - m| / T 2^-24 of itself, which a sum does not feel (what lies far below the maximum is little of it).
 __device__ __forceinline__ float td_term(float x, float m, float c) { return x == TD_NINF ? 0.f : td_exp2((x - m) * c); }
+
+// The same where each value counts by itself (a gradient's entry far below the maximum, a sum's factor): what the three roundings leave
+// out is carried along and multiplied on, so that the result is off by 5 steps of 2^-24 however far x lies below m.
+struct TdScale {
+    float c, low;  // log2(e) / T in two parts
+    __device__ __forceinline__ explicit TdScale(float temperature) {
+        constexpr float log2e_low = (float)(1.4426950408889634 - (double)TD_LOG2E);
+        c = TD_LOG2E / temperature;
+        low = (fmaf(-c, temperature, TD_LOG2E) + log2e_low) / temperature;
+    }
+    __device__ __forceinline__ float exp(float x, float m) const {  // (x = -inf: 0, where m is finite)
+        const float d = x - m, back = x - d, lost = (x - (d + back)) + (back - m);
+        const float t = d * c, rest = fmaf(lost, c, fmaf(d, low, fmaf(d, c, -t)));
+        return td_exp2(t) * __builtin_amdgcn_fmed3f(fmaf(rest, 0.69314718f, 1.f), 0.5f, 2.f);  // (rest is NaN where d is infinite)
+    }
+    __device__ __forceinline__ float term(float x, float m) const { return x == TD_NINF ? 0.f : exp(x, m); }
+};
 
 struct TdMaxOp { __device__ static float op(float a, float b) { return td_max(a, b); } };
 struct TdSumOp { __device__ static float op(float a, float b) { return a + b; } };
@@ -637,7 +655,7 @@ __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V,
                                               float scale, float m_r, float s_r, const TdSaved& out) {
     constexpr int Q = TD_MAX_K / WAVE;
     const int lane = lane_id();
-    const float c = TD_LOG2E / temperature;
+    const TdScale by_t(temperature);
     const bool with_rest = t.rest != nullptr;
     // (the rest is a logarithm of what has been divided by T; without it the difference is taken first)
     const float before = with_rest ? temperature : 1.f, after = with_rest ? 1.f : temperature;
@@ -710,14 +728,14 @@ __device__ __forceinline__ void td_finish_row(const T* __restrict__ zrow, int V,
             }
         first[q] = id[q] >= 0 && !(named >> lane & 1);
         if (id[q] >= 0) {
-            en[q] = td_term(zv[q], m, c);
+            en[q] = by_t.term(zv[q], m);
             if (first[q]) sn += en[q];
             else again += en[q];
             twice |= !first[q];
         }
     }
     sn = td_reduce_wave<TdSumOp>(sn);
-    const float rest_scale = td_term(m_r, m, c), su = s_r * rest_scale, s = sn + su;
+    const float rest_scale = by_t.term(m_r, m), su = s_r * rest_scale, s = sn + su;
     // loss
     const float log_ps = logf(ps), log_s = logf(s);
     float loss = -again / s;
@@ -898,9 +916,11 @@ __global__ __launch_bounds__(256) void k_top_distill_bwd(const T* __restrict__ z
     }
     const bool live = counted[row] != 0.f;
     const float gs = g[g_per_row ? row : 0] * scale / (divisor ? divisor[0] : 1.f);
-    const float c = TD_LOG2E / temperature;
+    const TdScale by_t(temperature);
     const float2 st = stats[row];
     const float f = gs * st.y;
+    // (the half types round far more away than the shorter form does)
+    auto gradient = [&](float x) { return (T)(f * (sizeof(T) == 4 ? by_t.exp(x, st.x) : td_exp2((x - st.x) * by_t.c))); };
     if (live) {
         for (int i = threadIdx.x; i <= (shift + len) / 32; i += blockDim.x) s_named[i] = 0;
         __syncthreads();
@@ -940,7 +960,7 @@ __global__ __launch_bounds__(256) void k_top_distill_bwd(const T* __restrict__ z
                 struct alignas(16) { T v[E]; } o;
                 td_unpack<T>(r[q], x);
 #pragma unroll
-                for (int e = 0; e < E; ++e) o.v[e] = live ? (T)(f * td_exp2((x[e] - st.x) * c)) : (T)0.f;
+                for (int e = 0; e < E; ++e) o.v[e] = live ? gradient(x[e]) : (T)0.f;
                 const uint32_t bits = live ? s_named[b >> 5] >> (b & 31) & ((1u << E) - 1u) : 0u;
                 if (bits == 0 && b >= shift && b + E <= shift + len) {
                     dg[v] = *reinterpret_cast<const uint4*>(&o);
@@ -954,7 +974,7 @@ __global__ __launch_bounds__(256) void k_top_distill_bwd(const T* __restrict__ z
     } else {
         for (int i = threadIdx.x; i < len; i += blockDim.x)
             if (!live) dp[i] = (T)0.f;
-            else if (!(s_named[i >> 5] >> (i & 31) & 1u)) dp[i] = (T)(f * td_exp2(((float)zp[i] - st.x) * c));
+            else if (!(s_named[i >> 5] >> (i & 31) & 1u)) dp[i] = gradient((float)zp[i]);
     }
 }
 

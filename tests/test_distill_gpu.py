@@ -542,6 +542,26 @@ def test_distill_place_named_twice_holds_nearly_all():
         assert bool(((d - want).abs()[heavy] <= U * steps * of_others).all())  # (as check_digits)
 
 
+@pytest.mark.parametrize("with_rest", [False, True])
+@pytest.mark.parametrize("V", [50, 1003, 40000])
+def test_distill_gradient_entries_far_below_the_maximum(V, with_rest):
+    """Two places that are not named have gradients in the ratio exp((z_v - z_w) / T): entries far below the largest keep their digits.  An
+    entry is off by a step for the exponential's own rounding (1 ulp is 2 steps of 2^-24), one each for 1 + the rest of the exponent, its
+    product, f and the product with it; two of them by 12, and the rest's own rounding is of second order.  (A temperature is a float32: 2.7
+    as a double is 1.8e-8 beside it, 60 times that in the exponent is 18 steps.)"""
+    for T in (0.5, 1.0, float(np.float32(2.7))):
+        z, ids, top, rest = make(5, V, 4, torch.float32, V, empty=0, with_rest=with_rest, T=T)
+        z = z + 7.3
+        z[:, ::3] -= torch.rand((5, z[:, ::3].shape[1]), generator=torch.Generator().manual_seed(V)) * 60.0 * T
+        d = grad_of_sum(z, ids, top, rest, T)
+        masked = z.double().scatter(1, ids.long(), -math.inf)
+        at = masked.argmax(1, keepdim=True)
+        want = torch.exp((masked - masked.gather(1, at)) / T)
+        seen = want > 1e-30  # (below: too near to the smallest normal number)
+        off = (d / d.gather(1, at) - want).abs() / want
+        assert bool((d.gather(1, at) != 0).all()) and float(off[seen].max()) <= 12 * U, float(off[seen].max()) / U
+
+
 def test_refusals_at_the_library():
     from samnerf_amd import _lib
     from samnerf_amd import _opcore as C
