@@ -4,7 +4,6 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._opcore import DTYPE_CODE, _dev, _L, _launch, _p, _rows, _stream_on
 
@@ -38,6 +37,17 @@ def _logits(t, name: str) -> None:
         raise ValueError(f"{name}: rows of 1 to {TOP_LOGITS_MAX_V} logits expected, got {tuple(t.shape)}")
 
 
+def _rows_in_place(t: torch.Tensor) -> bool:
+    """Whether `_rows(t)` is a view."""
+    if t.is_contiguous():
+        return True
+    try:
+        m = t.detach().view(-1, t.shape[-1]) if t.dim() != 2 else t
+    except RuntimeError:
+        return False
+    return not (m.shape[1] > 1 and m.stride(1) != 1 or m.shape[0] > 1 and m.stride(0) < m.shape[1])
+
+
 def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty((nbytes // 8,), device=device, dtype=torch.int64) if nbytes else None
 
@@ -66,6 +76,17 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     return TopLogits(ids, vals, rest)
 
 
+class _OnceDifferentiable(torch.autograd.Function):
+    # the gradient as a function of what it depends on, for create_graph: asking for its derivative is refused, not answered with nothing
+    @staticmethod
+    def forward(ctx, student, g, first):
+        return _TopDistill._gradient(first, g)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("top_logits_distill_loss has no second derivative (its gradient was differentiated)")
+
+
 class _TopDistill(torch.autograd.Function):
     # one buffer of floats: stats [R, 2], diff [R, K], counted [R], the divisor, rows [R] (unless they are the result)
     @staticmethod
@@ -90,20 +111,19 @@ class _TopDistill(torch.autograd.Function):
                     int(reduction == "mean"), None if per_row else _p(loss), divisor, _p(ws), nbytes, _stream_on(student.get_device()),
                     units=float(R * V * z.element_size()))
         ctx.args = (student.shape, R, V, ld, K, temperature, weight, per_row)
-        ctx.save_for_backward(z, ids, saved)
+        ctx.save_for_backward(z, ids, saved, student)
         return loss
 
     @staticmethod
     def backward(ctx, g):
-        if torch.is_grad_enabled():  # create_graph: a second derivative is refused when it is asked for
-            return _TopDistill._refusing_twice(ctx, g)
-        return _TopDistill._gradient(ctx, g)
+        dz = None
+        if ctx.needs_input_grad[0]:
+            dz = _OnceDifferentiable.apply(ctx.saved_tensors[3], g, ctx) if torch.is_grad_enabled() else _TopDistill._gradient(ctx, g)
+        return dz, None, None, None, None, None, None
 
     @staticmethod
     def _gradient(ctx, g):
-        if not ctx.needs_input_grad[0]:
-            return (None,) * 7
-        z, ids, saved = ctx.saved_tensors
+        z, ids, saved, _ = ctx.saved_tensors
         shape, R, V, ld, K, temperature, weight, per_row = ctx.args
         dz = torch.empty(shape, device=z.device, dtype=z.dtype)
         if R:
@@ -114,9 +134,7 @@ class _TopDistill(torch.autograd.Function):
             _launch("snf_top_distill_bwd", _p(z), DTYPE_CODE[z.dtype], R, V, ld, _p(ids), int(ids.dtype == torch.int64), K, temperature,
                     weight, _p(g), int(per_row), None if per_row else divisor, counted, at, at + 8 * R, _p(dz), _stream_on(z.get_device()),
                     units=float(2 * R * V * z.element_size()))
-        return dz, None, None, None, None, None, None
-
-    _refusing_twice = staticmethod(once_differentiable(_gradient.__func__))
+        return dz
 
 
 def top_logits_distill_loss(student: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor, rest: Optional[torch.Tensor] = None,
@@ -128,7 +146,7 @@ def top_logits_distill_loss(student: torch.Tensor, ids: torch.Tensor, logits: to
     against the student's mass on all places that the ids do not name; without it the teacher's probabilities sum to 1 over the list.
     reduction "mean": over the rows with a target (a row without entries, or whose teacher has no mass, has none; no such row: 0); "sum";
     "none": [...] float32.  An id named twice counts twice for the teacher; an id >= V makes its row NaN.  The teacher's tensors get no
-    gradient.  K <= 256.  (To capture the backward pass into a graph, let no eager graph of the same leaves live: autograd would
+    gradient, and the gradient has no derivative of its own (a RuntimeError).  K <= 256.  (To capture the backward pass into a graph, let no eager graph of the same leaves live: autograd would
     accumulate on that graph's stream.)"""
     _logits(student, "student")
     _logits(logits, "logits")
@@ -157,4 +175,6 @@ def top_logits_distill_loss(student: torch.Tensor, ids: torch.Tensor, logits: to
         _dev(rest, "rest", di)
         if rest.requires_grad:
             rest = rest.detach()
+    if not _rows_in_place(student):  # (copied here, not within: what is kept for the backward pass is then the copy alone)
+        student = student.contiguous()
     return _TopDistill.apply(student, ids, logits, rest, t, float(weight), reduction)

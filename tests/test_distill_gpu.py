@@ -562,6 +562,62 @@ def test_distill_gradient_entries_far_below_the_maximum(V, with_rest):
         assert bool((d.gather(1, at) != 0).all()) and float(off[seen].max()) <= 12 * U, float(off[seen].max()) / U
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_distill_second_derivative_is_refused(reduction):
+    """With create_graph the gradient is what it is without, and part of the graph: a term of a loss that holds it cannot be dropped."""
+    from samnerf_amd import ops
+    z, ids, top, rest = (t.cuda() for t in make(6, 90, 5, torch.float32, 4, empty=0))
+    views = (lambda x: x, lambda x: x.view(2, 3, 90), lambda x: x[:1].expand(6, 90), lambda x: x.t().contiguous().t())
+    for view in views:
+        x = z.clone().requires_grad_(True)
+        s = view(x)
+        lead = s.shape[:-1]
+
+        def loss_of():
+            return ops.top_logits_distill_loss(s, ids.view(*lead, 5), top.view(*lead, 5), rest=rest.view(lead), reduction=reduction).sum()
+
+        (want,) = torch.autograd.grad(loss_of(), x)
+        loss = loss_of()
+        (g,) = torch.autograd.grad(loss, x, create_graph=True)
+        assert torch.equal(g, want) and not want.requires_grad and g.requires_grad
+        for what in (lambda: loss + g.pow(2).sum(), lambda: g.sum()):
+            with pytest.raises(RuntimeError, match="no second derivative"):
+                what().backward()
+            loss = loss_of()
+            (g,) = torch.autograd.grad(loss, x, create_graph=True)
+    scale = torch.ones((), device="cuda", requires_grad=True)  # an incoming gradient that requires one
+    x = z.clone().requires_grad_(True)
+    loss = scale * ops.top_logits_distill_loss(x, ids, top, rest=rest)
+    (g,) = torch.autograd.grad(loss, x, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(g.sum(), scale)
+
+
+def test_distill_student_written_after_the_call():
+    """Where the call has copied the student (its rows are not contiguous), writing the original afterwards changes nothing; a student that
+    is read in place again by the backward pass must not be written."""
+    from samnerf_amd import ops
+    z, ids, top, rest = (t.cuda() for t in make(6, 90, 5, torch.float32, 4, empty=0))
+    for view in (lambda x: x.t().contiguous().t(), lambda x: x.view(2, 3, 90).permute(0, 2, 1).contiguous().permute(0, 2, 1)):
+        x = z.clone().requires_grad_(True)
+        s = view(x)
+        lead = s.shape[:-1]
+        args = (ids.view(*lead, 5), top.view(*lead, 5), rest.view(lead))
+        (want,) = torch.autograd.grad(ops.top_logits_distill_loss(s, *args), x)
+        s = view(x)
+        loss = ops.top_logits_distill_loss(s, *args)
+        with torch.no_grad():
+            s.zero_()
+        assert torch.equal(torch.autograd.grad(loss, x)[0], want)
+    x = z.clone().requires_grad_(True)
+    s = x * 1.0
+    loss = ops.top_logits_distill_loss(s, ids, top, rest)
+    with torch.no_grad():
+        s.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+
+
 def test_refusals_at_the_library():
     from samnerf_amd import _lib
     from samnerf_amd import _opcore as C
