@@ -523,7 +523,7 @@ int snf_attention_planes_rp(const float* qkv, const float* rel_pos_h, const floa
  *   [R, K] of top_dtype, rest [R] or NULL.  With p = softmax over the row's entries of (top / T [, rest]), q = softmax(z / T), q_rest =
  *   sum of q over the places that the row's ids do not name:
  *     rows[r] = weight T^2 ( sum_k p_k (log p_k - log q_ids_k) + p_rest (log p_rest - log q_rest) )
- *   without rest, p sums to 1 over the entries.  Rows without an entry, or whose teacher has no mass, are no targets: rows = counted = 0.
+ *   without rest, p sums to 1 over the entries.  weight and weight T^2 are 0 or normal numbers.  Rows without an entry, or whose teacher has no mass, are no targets: rows = counted = 0.
  *   An id >= V makes its row NaN.  stats [R, 2] (8-byte aligned) and diff [R, K] are kept for the backward pass.  loss (or NULL) [1] = sum of
  *   rows / divisor[0], divisor [1] = number of counted rows (at least 1) or, mean == 0, 1.  workspace:
  *   snf_top_distill_workspace_bytes(...) bytes, 8-byte aligned.

@@ -1046,12 +1046,18 @@ static int td_top_t(const T* x, int R, int V, int64_t ld, int k, float temperatu
     return SNF_OK;
 }
 
+// weight and weight T^2, which the rows' divergences are multiplied by: 0 or a normal number (weight T, the gradient's factor, is between)
+static bool td_weight_ok(float weight, float temperature) {
+    const double w = fabs((double)weight), scale = w * temperature * temperature;
+    return weight == 0.f || (w >= FLT_MIN && w <= FLT_MAX && scale >= FLT_MIN && scale <= FLT_MAX);
+}
+
 template <typename T>
 static int td_fwd_t(const T* z, int R, int V, int64_t ld, const TdTeacher& t, float temperature, float weight, const TdSaved& out, void* ws,
                     hipStream_t st) {
     const TdPlan pl = td_rows_plan(R, V, 16 / (int)sizeof(T));
     SNF_REQUIRE((int64_t)R * pl.parts * TD_SHAPES[pl.shape].threads < ((int64_t)1 << 32), "snf_top_distill_fwd: %d rows of %d are too many for one launch", R, V);
-    const float scale = weight * temperature * temperature;
+    const float scale = (float)((double)weight * temperature * temperature);
     const dim3 grid((unsigned)((int64_t)R * pl.parts));
 #define TD_GO(S_)                                                                                                                     \
     case S_:                                                                                                                          \
@@ -1134,6 +1140,8 @@ int snf_top_distill_fwd(const void* z, int dtype, int R, int V, int64_t ld, cons
     SNF_REQUIRE(R >= 0 && V >= 1 && V <= SNF_TOP_MAX_V, "snf_top_distill_fwd: bad sizes R=%d V=%d", R, V);
     SNF_REQUIRE(K >= 1 && K <= snf::TD_MAX_K, "snf_top_distill_fwd: K=%d is not in 1 .. %d", K, snf::TD_MAX_K);
     SNF_REQUIRE(temperature >= FLT_MIN && temperature < INFINITY, "snf_top_distill_fwd: temperature %g", (double)temperature);
+    SNF_REQUIRE(snf::td_weight_ok(weight, temperature), "snf_top_distill_fwd: weight %g (T %g): it and weight T^2 are 0 or normal numbers",
+                (double)weight, (double)temperature);
     SNF_REQUIRE(dtype >= SNF_F32 && dtype <= SNF_F16 && top_dtype >= SNF_F32 && top_dtype <= SNF_F16, "snf_top_distill_fwd: unknown dtype");
     SNF_REQUIRE(!loss || divisor, "snf_top_distill_fwd: null pointer");
     hipStream_t st = (hipStream_t)stream;
@@ -1157,6 +1165,8 @@ int snf_top_distill_bwd(const void* z, int dtype, int R, int V, int64_t ld, cons
     SNF_REQUIRE(R >= 0 && V >= 1 && V <= SNF_TOP_MAX_V, "snf_top_distill_bwd: bad sizes R=%d V=%d", R, V);
     SNF_REQUIRE(K >= 1 && K <= snf::TD_MAX_K, "snf_top_distill_bwd: K=%d is not in 1 .. %d", K, snf::TD_MAX_K);
     SNF_REQUIRE(temperature >= FLT_MIN && temperature < INFINITY, "snf_top_distill_bwd: temperature %g", (double)temperature);
+    SNF_REQUIRE(snf::td_weight_ok(weight, temperature), "snf_top_distill_bwd: weight %g (T %g): it and weight T^2 are 0 or normal numbers",
+                (double)weight, (double)temperature);
     SNF_REQUIRE(dtype >= SNF_F32 && dtype <= SNF_F16, "snf_top_distill_bwd: unknown dtype %d", dtype);
     if (R == 0) return SNF_OK;
     SNF_REQUIRE(z && ids && g && counted && stats && diff && dz, "snf_top_distill_bwd: null pointer");

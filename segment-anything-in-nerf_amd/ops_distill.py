@@ -1,6 +1,7 @@
 """A teacher's top logits and the distillation loss that reads them (csrc/distill.hip); `samnerf_amd.ops` re-exports everything here."""
 from __future__ import annotations
 
+from ctypes import c_float
 from typing import NamedTuple, Optional
 
 import torch
@@ -25,9 +26,18 @@ class TopLogits(NamedTuple):
 
 def _temperature(t) -> float:
     t = float(t)
-    if not 2.0 ** -126 <= t < 2.0 ** 128:
+    if not 2.0 ** -126 <= t <= 3.4028234663852886e38:
         raise ValueError(f"temperature: a positive normal float32 expected, got {t}")
-    return t
+    return c_float(t).value
+
+
+def _weight(w, t: float) -> float:
+    # the loss is a row's divergence times weight T^2: 0, or within float32's normal numbers
+    w = float(w)
+    scale = abs(c_float(w).value) * t * t
+    if w != 0.0 and not (2.0 ** -126 <= abs(w) < 2.0 ** 128 and 2.0 ** -126 <= scale < 2.0 ** 128):
+        raise ValueError(f"weight, temperature: weight and weight T^2 have to be 0 or normal float32 numbers, got {w} and {scale}")
+    return w
 
 
 def _logits(t, name: str) -> None:
@@ -147,10 +157,11 @@ def top_logits_distill_loss(student: torch.Tensor, ids: torch.Tensor, logits: to
     reduction "mean": over the rows with a target (a row without entries, or whose teacher has no mass, has none; no such row: 0); "sum";
     "none": [...] float32.  An id named twice counts twice for the teacher; an id >= V makes its row NaN.  The teacher's tensors get no
     gradient, and the gradient has no derivative of its own (a RuntimeError).  K <= 256.  (To capture the backward pass into a graph, let no eager graph of the same leaves live: autograd would
-    accumulate on that graph's stream.)"""
+    accumulate on that graph's stream.)  weight and weight T^2 are 0 or normal float32 numbers."""
     _logits(student, "student")
     _logits(logits, "logits")
     t = _temperature(temperature)
+    w = _weight(weight, t)
     lead = student.shape[:-1]
     if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"ids: int32 or int64 expected, got {getattr(ids, 'dtype', type(ids))}")
@@ -177,4 +188,4 @@ def top_logits_distill_loss(student: torch.Tensor, ids: torch.Tensor, logits: to
             rest = rest.detach()
     if not _rows_in_place(student):  # (copied here, not within: what is kept for the backward pass is then the copy alone)
         student = student.contiguous()
-    return _TopDistill.apply(student, ids, logits, rest, t, float(weight), reduction)
+    return _TopDistill.apply(student, ids, logits, rest, t, w, reduction)

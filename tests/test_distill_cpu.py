@@ -89,3 +89,32 @@ def test_the_library_refuses_before_any_launch():
         refused(fwd(**kw), word)
     refused(lib.snf_top_distill_bwd(p, 0, 4, 64, 64, p, 0, 3, 1.0, 1.0, None, 0, None, p, p, p, p, None), b"null")
     refused(lib.snf_top_distill_bwd(p, 9, 4, 64, 64, p, 0, 3, 1.0, 1.0, p, 0, None, p, p, p, p, None), b"dtype")
+
+
+def test_distill_loss_refuses_scales_outside_float32():
+    """weight T^2 multiplies every row: where it is no normal float32 (and not 0) the loss would be infinite, NaN or 0 beside a finite
+    gradient."""
+    from samnerf_amd import _lib, ops
+    z, ids, top, rest = _args()
+    f = ops.top_logits_distill_loss
+    lib = _lib.load()
+    p = 4096  # an aligned address that is never followed
+
+    def library(w, T):
+        a = lib.snf_top_distill_fwd(None, 0, 4, 64, 64, None, 0, None, 0, None, 3, T, w, p, p, p, p, 0, None, None, None, 0, None)
+        first = lib.snf_last_error()
+        b = lib.snf_top_distill_bwd(None, 0, 4, 64, 64, None, 0, 3, T, w, None, 0, None, p, p, p, p, None)
+        assert a == b == -1 and (b"weight" in first) == (b"weight" in lib.snf_last_error())
+        return b"weight" in first  # (else: a null pointer)
+
+    inside = ((1.0, 1.8e19), (1.0, 1.1e-19), (1e30, 1e4), (-1e-30, 1.1e-4), (0.0, 3e38), (0.0, 2e-38), (-2.0, 1.0), (3.4e38, 1.0), (1.2e-38, 1.0))
+    outside = ((1.0, 1.9e19), (1.0, 1e-19), (1e30, 2e4), (-1e-30, 1e-4), (1e-40, 1e10), (1.0, 3e38), (float("nan"), 1.0), (float("inf"), 1.0),
+               (3.5e38, 1.0))
+    for w, T in inside:
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            f(z, ids, top, rest=rest, temperature=T, weight=w)
+        assert not library(w, T)
+    for w, T in outside:
+        with pytest.raises(ValueError, match="weight"):
+            f(z, ids, top, rest=rest, temperature=T, weight=w)
+        assert library(w, T)

@@ -618,6 +618,32 @@ def test_distill_student_written_after_the_call():
         loss.backward()
 
 
+@pytest.mark.parametrize("with_rest", [False, True])
+@pytest.mark.parametrize("T,weight", [(1.7e19, 1.0), (2e-19, 1.0), (1e15, 1e-30), (1e-15, 1e30), (2.0, 0.0)])
+def test_distill_at_the_ends_of_the_scale(T, weight, with_rest):
+    """Temperatures and weights whose weight T^2 is just inside float32, logits of the temperature's size: the loss and the gradient of the
+    same rows at T near 1, scaled."""
+    z, ids, top, rest = make(5, 60, 4, torch.float32, 8, empty=0, with_rest=with_rest)
+    # logits at the temperature's size; the rest has been divided by it
+    k = 2.0 ** round(math.log2(T))
+    Tk = T / k
+    from samnerf_amd import ops
+    x = (z * k).cuda().requires_grad_(True)
+    a = dict(rest=rest.cuda() if with_rest else None, reduction="none")
+    got = ops.top_logits_distill_loss(x, ids.cuda(), (top * k).cuda(), temperature=T, weight=weight, **a)
+    (g,) = torch.autograd.grad(got, x, torch.ones_like(got))
+    y = z.cuda().requires_grad_(True)
+    want = ops.top_logits_distill_loss(y, ids.cuda(), top.cuda(), temperature=Tk, weight=1.0, **a)
+    (h,) = torch.autograd.grad(want, y, torch.ones_like(want))
+    # powers of two move nothing but the scale: T = k Tk to a rounding of T (exponents up to 20, as many steps), weight T^2 and weight T to one
+    scale = weight * T * T / (Tk * Tk)
+    over = want.double() * scale > torch.finfo(torch.float32).max  # a loss that no float32 holds: infinite
+    assert bool(torch.isfinite(g).all()) and torch.equal(torch.isinf(got), over) and not bool(torch.isnan(got).any())
+    got = torch.where(over, want.double() * scale, got.double())
+    assert bool(((got - want.double() * scale).abs() <= 60 * U * abs(scale) * (want.double().abs() + Tk * Tk)).all())
+    assert bool(((g.double() - h.double() * (weight * k)).abs() <= 60 * U * weight * k * Tk * 2).all())
+
+
 def test_refusals_at_the_library():
     from samnerf_amd import _lib
     from samnerf_amd import _opcore as C
