@@ -45,6 +45,8 @@ def _logits(t, name: str) -> None:
         raise TypeError(f"{name}: float32, bfloat16 or float16 expected, got {getattr(t, 'dtype', type(t))}")
     if t.dim() < 1 or not 1 <= t.shape[-1] <= TOP_LOGITS_MAX_V:
         raise ValueError(f"{name}: rows of 1 to {TOP_LOGITS_MAX_V} logits expected, got {tuple(t.shape)}")
+    if t.numel() // t.shape[-1] >= 1 << 31:  # (the library counts rows in 32 bits)
+        raise ValueError(f"{name}: fewer than 2^31 rows expected, got {tuple(t.shape)}")
 
 
 def _rows_in_place(t: torch.Tensor) -> bool:

@@ -118,3 +118,14 @@ def test_distill_loss_refuses_scales_outside_float32():
         with pytest.raises(ValueError, match="weight"):
             f(z, ids, top, rest=rest, temperature=T, weight=w)
         assert library(w, T)
+
+
+def test_row_counts_past_32_bits_are_refused():
+    """2^32 + 3 rows are not 3."""
+    from samnerf_amd import ops
+    n = 2 ** 32 + 3
+    x = torch.zeros((1, 1)).expand(n, 1)
+    with pytest.raises(ValueError, match="rows"):
+        ops.top_logits(x, 1)
+    with pytest.raises(ValueError, match="rows"):
+        ops.top_logits_distill_loss(x, torch.zeros((1, 1), dtype=torch.int32).expand(n, 1), x)
