@@ -102,7 +102,8 @@ class ImageEncoderViT(nn.Module):
                                      rel_pos_zero_init=rel_pos_zero_init,
                                      window_size=window_size if i not in global_attn_indexes else 0,
                                      input_size=(img_size // patch_size, img_size // patch_size)))
-        self._wcache, self._pcache = {}, {}  # split weights / operand-plane buffers of the split-operand block path
+        self._wcache, self._pcache = {}, {}  # split and quantised weights / operand-plane buffers of the split-operand block path, by stream
+        self._wcaptured = {}  # weights that captured forwards read
         self.linear_format = "split"
         self.neck = nn.Sequential(nn.Conv2d(embed_dim, out_chans, kernel_size=1, bias=False), LayerNorm2d(out_chans),
                                   nn.Conv2d(out_chans, out_chans, kernel_size=3, padding=1, bias=False),
@@ -139,55 +140,74 @@ class ImageEncoderViT(nn.Module):
         h = ops.linear_mxfp4(x, self._wmxfp4(mlp.lin1), mlp.lin1.bias, ops.ACT_GELU, quantized=True)
         return ops.linear_mxfp4(h, self._wmxfp4(mlp.lin2), mlp.lin2.bias)
 
-    def _wmxfp4(self, lin) -> "ops.Mxfp4":
-        """A layer's quantised weight, once per write of the parameter (as _wplanes)."""
-        key, tag = (id(lin.weight), "mxfp4"), (lin.weight._version, lin.weight.data_ptr(), str(lin.weight.device))
-        hit = self._wcache.get(key)
+    def _wcached(self, lin, kind, make):
+        """A layer's weight in the form `make` gives it, once per write of the parameter (load_state_dict; writes through `.data` bump no
+        version: call reset_weight_cache() after those).  What is kept is whole before it is kept, so that every stream may read it, and what
+        it replaces is not read any more.  A capture that finds nothing makes its own, in the graph; one that finds something keeps it alive,
+        whatever is written afterwards."""
+        key, tag = (id(lin.weight), kind), (lin.weight._version, lin.weight.data_ptr(), str(lin.weight.device))
+        hit, capturing = self._wcache.get(key), torch.cuda.is_current_stream_capturing()
         if hit is None or hit[0] != tag:
-            hit = self._wcache[key] = (tag, ops.quantize_mxfp4(lin.weight.detach().float()))
+            hit = (tag, make(lin.weight.detach().float().contiguous()))
+            if not capturing:
+                torch.cuda.synchronize(lin.weight.device)
+                self._wcache[key] = hit
+        elif capturing:
+            self._wcaptured[id(hit)] = hit
         return hit[1]
 
+    def _wmxfp4(self, lin) -> "ops.Mxfp4":
+        """A layer's quantised weight."""
+        return self._wcached(lin, "mxfp4", ops.quantize_mxfp4)
+
     def _wplanes(self, lin, M: int = 0):
-        """bf16 hi / lo planes of a layer's weight, split once and re-split when the parameter is written (load_state_dict).
+        """bf16 hi / lo planes of a layer's weight.
         M (rows of the product) given: k-blocked planes where 256 x 320 tiles fill the chip in one round -- the GEMM with both
         operands through LDS (ViT-H: attn.qkv, mlp.lin1; SNF_VIT_GEMM_LDS=0: never)."""
         Nc, K = lin.weight.shape
         kb = bool(M) and _GEMM_LDS and K % 64 == 0 and Nc % 320 == 0 and 160 <= -(-M // 256) * (Nc // 320) <= 256
-        key, tag = (id(lin.weight), kb), (lin.weight._version, lin.weight.data_ptr(), str(lin.weight.device))
-        hit = self._wcache.get(key)
-        if hit is None or hit[0] != tag:  # (writes through `.data` bump no version: call reset_weight_cache() after those)
-            w = lin.weight.detach().float().contiguous()
-            hit = (tag, ops.split_weight_planes_kb(w) if kb else ops.split_weight_planes(w))
-            self._wcache[key] = hit
-        return hit[1]
+        return self._wcached(lin, kb, ops.split_weight_planes_kb if kb else ops.split_weight_planes)
+
+    def _forget_weights(self) -> None:
+        if self._wcache:
+            torch.cuda.synchronize()  # (a stream may still read them)
+            self._wcache.clear()
 
     def reset_weight_cache(self) -> None:
-        """Forget the split weights (after changing parameters in a way autograd's version counter does not see)."""
-        self._wcache.clear()
+        """Forget the split and quantised weights (after changing parameters in a way autograd's version counter does not see), also those
+        that captured forwards read: such a graph is captured again, not replayed."""
+        self._forget_weights()
+        self._wcaptured.clear()
 
     # `.data` writes bump no version counter: the two module-level ways parameters are replaced wholesale drop the cache themselves
     def _apply(self, fn, *args, **kw):
-        self._wcache.clear()
+        self._forget_weights()
         self._pcache.clear()
         return super()._apply(fn, *args, **kw)
 
     def load_state_dict(self, *args, **kw):
-        self._wcache.clear()
+        self._forget_weights()
         return super().load_state_dict(*args, **kw)
 
     def _load_from_state_dict(self, *args, **kw):
         # (reached when the state is loaded through a PARENT module, e.g. `sam.load_state_dict`, which never calls the override above)
-        self._wcache.clear()
+        self._forget_weights()
         return super()._load_from_state_dict(*args, **kw)
 
-    def _pbuf(self, tag: str, M: int, K: int, device, zero: bool = False):
-        key = (tag, M, K, str(device))
-        buf = self._pcache.get(key)
+    def _pbufs(self, device) -> dict:
+        """The operand-plane buffers of a forward: those of its stream, or, while it is captured, the graph's own."""
+        if torch.cuda.is_current_stream_capturing():
+            return {}
+        return self._pcache.setdefault((str(device), torch.cuda.current_stream(device).cuda_stream), {})
+
+    @staticmethod
+    def _pbuf(bufs: dict, tag: str, M: int, K: int, device, zero: bool = False):
+        buf = bufs.get((tag, M, K))
         if buf is None:
-            buf = self._pcache[key] = ops.Planes.empty(M, K, device, zero=zero)
+            buf = bufs[(tag, M, K)] = ops.Planes.empty(M, K, device, zero=zero)
         return buf
 
-    def _block_planes(self, blk, shortcut, pending, B: int, G: int):
+    def _block_planes(self, blk, shortcut, pending, B: int, G: int, bufs: dict):
         """Block.forward (image_encoder.py:164-182) with every GEMM operand born split: norm1 writes qkv's operand at the window
         partition's rows, the attention writes proj's, norm2 lin1's, lin1's GELU epilogue lin2's."""
         a, ws, dev = blk.attn, blk.window_size, shortcut.device
@@ -195,11 +215,11 @@ class ImageEncoderViT(nn.Module):
         if ws > 0:
             nW = (G + ws - 1) // ws
             n, Bw = ws, B * nW * nW
-            y = self._pbuf("n1w", Bw * ws * ws, C, dev, zero=True)  # padded rows: written by nobody, zero for good
+            y = self._pbuf(bufs, "n1w", Bw * ws * ws, C, dev, zero=True)  # padded rows: written by nobody, zero for good
             grid = (G, G, ws)
         else:
             n, Bw = G, B
-            y = self._pbuf("n1", B * G * G, C, dev)
+            y = self._pbuf(bufs, "n1", B * G * G, C, dev)
             grid = None
         if pending is None:
             ops.layernorm_planes(shortcut, blk.norm1.weight, blk.norm1.bias, blk.norm1.eps, y, grid=grid)
@@ -208,11 +228,11 @@ class ImageEncoderViT(nn.Module):
                                                want_sum=True, grid=grid)
         mx = self.linear_format == "mxfp4"
         qkv = ops.linear_mxfp4(y, self._wmxfp4(a.qkv), a.qkv.bias) if mx else ops.linear_planes(y, self._wplanes(a.qkv, y.M), a.qkv.bias)
-        o = ops.attention_planes(qkv, Bw, n * n, a.num_heads, n, self._pbuf("att", Bw * n * n, C, dev),
+        o = ops.attention_planes(qkv, Bw, n * n, a.num_heads, n, self._pbuf(bufs, "att", Bw * n * n, C, dev),
                                  a.rel_pos_h if a.use_rel_pos else None, a.rel_pos_w if a.use_rel_pos else None)
         o = ops.linear_mxfp4(o, self._wmxfp4(a.proj), a.proj.bias) if mx else ops.linear_planes(o, self._wplanes(a.proj), a.proj.bias)
         # x = shortcut + window_unpartition(proj) inside norm2 (its residual input, read at the token's window row)
-        n2 = self._pbuf("n2", B * G * G, C, dev)
+        n2 = self._pbuf(bufs, "n2", B * G * G, C, dev)
         if ws > 0:
             y2, shortcut = ops.layernorm_planes_merge(shortcut, o, blk.norm2.weight, blk.norm2.bias, blk.norm2.eps, n2, B, G, G, ws)
         else:
@@ -220,7 +240,7 @@ class ImageEncoderViT(nn.Module):
         if mx:
             return shortcut, self._mlp_mxfp4(blk.mlp, y2)
         h = ops.linear_planes(y2, self._wplanes(blk.mlp.lin1, y2.M), blk.mlp.lin1.bias, ops.ACT_GELU,
-                              out=self._pbuf("h", B * G * G, Mh, dev))
+                              out=self._pbuf(bufs, "h", B * G * G, Mh, dev))
         pending = ops.linear_planes(h, self._wplanes(blk.mlp.lin2), blk.mlp.lin2.bias)
         return shortcut, pending
 
@@ -239,6 +259,7 @@ class ImageEncoderViT(nn.Module):
                               pe.bias)
         if self.pos_embed is not None:
             t = t.view(B, T, -1).add_(self.pos_embed.view(1, T, -1)).view(B * T, -1)
+        bufs = self._pbufs(t.device)
         shortcut, pending = t, None  # `pending`: the previous block's MLP output, still to be added to `shortcut`
         trace = {}
         if -1 in trace_blocks:
@@ -246,7 +267,7 @@ class ImageEncoderViT(nn.Module):
         for bi, blk in enumerate(self.blocks):
             a, ws = blk.attn, blk.window_size
             if self._planes_ok(blk):
-                shortcut, pending = self._block_planes(blk, shortcut, pending, B, G)
+                shortcut, pending = self._block_planes(blk, shortcut, pending, B, G, bufs)
                 if bi in trace_blocks:
                     trace[bi] = ops.window_merge_add(pending, shortcut, B, G, G, 0).view(B, G, G, -1)
                 continue

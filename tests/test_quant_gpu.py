@@ -433,3 +433,68 @@ def test_encoder_weights_are_requantised_when_written():
     assert torch.equal(enc(x), a)
     with pytest.raises(ValueError):
         enc.set_linear_format("fp4")
+
+
+@pytest.mark.parametrize("fmt", ["split", "mxfp4"])
+def test_encoder_on_two_streams(fmt):
+    """A first forward on a busy stream and one on another right behind it, and forwards of both streams at once: each as alone (weights
+    that a cache holds are whole, operand planes are a stream's own)."""
+    enc = _small_encoder(256).set_linear_format(fmt)
+    g = torch.Generator().manual_seed(1)
+    xs = [torch.randn((1, 3, 224, 224), generator=g).cuda() for _ in range(4)]
+    want = [enc(x) for x in xs]
+    enc.reset_weight_cache()
+    side = torch.cuda.Stream()
+    a = torch.randn((4096, 4096), device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            a = (a @ a).clamp_(-1.0, 1.0)
+        first = enc(xs[0])
+    second = enc(xs[1])
+    torch.cuda.synchronize()
+    assert torch.equal(first, want[0]) and torch.equal(second, want[1])
+    got = []
+    for i in range(12):
+        with torch.cuda.stream(side):
+            got.append((2 * (i % 2), enc(xs[2 * (i % 2)])))
+        got.append((2 * (i % 2) + 1, enc(xs[2 * (i % 2) + 1])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+
+
+@pytest.mark.parametrize("cold", [True, False])
+@pytest.mark.parametrize("fmt", ["split", "mxfp4"])
+@pytest.mark.parametrize("embed", [64, 256])
+def test_encoder_captured(embed, fmt, cold):
+    """A captured forward replays as the eager one, with eager forwards in between; one captured before anything was cached leaves nothing in
+    the cache that only its replays write; one that read the cache keeps what it read, also after the weights were written."""
+    enc = _small_encoder(embed).set_linear_format(fmt)
+    g = torch.Generator().manual_seed(2)
+    xs = [torch.randn((1, 3, 224, 224), generator=g).cuda() for _ in range(3)]
+    want = [enc(x) for x in xs]
+    if cold:
+        enc.reset_weight_cache()
+        enc._pcache.clear()
+    torch.cuda.synchronize()
+    x = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = enc(x)
+    assert torch.equal(enc(xs[1]), want[1])  # before any replay
+    for i in (2, 0, 1):
+        x.copy_(xs[i])
+        graph.replay()
+        eager = enc(xs[(i + 1) % 3])
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[i]) and torch.equal(eager, want[(i + 1) % 3])
+    cached = fmt == "mxfp4" or embed == 256  # (the plain path of the other format reads the parameters themselves)
+    with torch.no_grad():
+        enc.blocks[0].attn.qkv.weight.mul_(0.5)
+    new = enc(xs[1])
+    junk = [torch.full((1 << 22,), float("nan"), device="cuda") for _ in range(8)]  # (what was freed is written again)
+    graph.replay()
+    torch.cuda.synchronize()
+    del junk
+    assert not torch.equal(new, want[1])
+    assert torch.equal(y, want[1] if cached and not cold else new)
