@@ -145,16 +145,17 @@ class ImageEncoderViT(nn.Module):
         version: call reset_weight_cache() after those).  What is kept is whole before it is kept, so that every stream may read it, and what
         it replaces is not read any more.  A capture that finds nothing makes its own, in the graph; one that finds something keeps it alive,
         whatever is written afterwards."""
-        key, tag = (id(lin.weight), kind), (lin.weight._version, lin.weight.data_ptr(), str(lin.weight.device))
+        w = lin.weight  # (kept with its form: the address and the version of another parameter may be those of one that is gone)
+        key, tag = (id(lin), kind), (w._version, w.data_ptr(), str(w.device))
         hit, capturing = self._wcache.get(key), torch.cuda.is_current_stream_capturing()
-        if hit is None or hit[0] != tag:
-            hit = (tag, make(lin.weight.detach().float().contiguous()))
+        if hit is None or hit[0] is not w or hit[1] != tag:
+            hit = (w, tag, make(w.detach().float().contiguous()))
             if not capturing:
-                torch.cuda.synchronize(lin.weight.device)
+                torch.cuda.synchronize(w.device)
                 self._wcache[key] = hit
         elif capturing:
             self._wcaptured[id(hit)] = hit
-        return hit[1]
+        return hit[2]
 
     def _wmxfp4(self, lin) -> "ops.Mxfp4":
         """A layer's quantised weight."""

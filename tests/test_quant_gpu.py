@@ -498,3 +498,17 @@ def test_encoder_captured(embed, fmt, cold):
     del junk
     assert not torch.equal(new, want[1])
     assert torch.equal(y, want[1] if cached and not cold else new)
+
+
+def test_encoder_weights_that_are_replaced():
+    """A new parameter in a layer is a new weight, also where it lies at the address of an earlier one that is gone."""
+    from samnerf_amd import ops
+    enc = _small_encoder(64)
+    lin = enc.blocks[0].attn.qkv
+    shape = lin.weight.shape
+    for i in range(40):
+        lin.weight = None
+        lin.weight = torch.nn.Parameter(torch.full(shape, float(i + 1), device="cuda"))
+        assert torch.equal(enc._wmxfp4(lin).float(), ops.quantize_mxfp4(lin.weight.detach()).float())
+        hi, lo = enc._wplanes(lin)
+        assert bool((hi.float() + lo.float() == i + 1).all())
