@@ -82,7 +82,8 @@ class Mxfp4:
 def quantize_mxfp4(x: Union[torch.Tensor, Planes]) -> Mxfp4:
     """x [..., K] (float32 / bfloat16 / float16; rows may be strided; or the encoder's operand planes) -> Mxfp4.  Per block of 32 along K the scale is
     2^max(floor(log2 max|x|) - 2, -127); values are rounded to the nearest code (halves to even), magnitudes above 6 scales become 6.
-    Blocks with an infinity or a NaN become NaN as a whole.  The last block of a K that 32 does not divide is filled with zeros."""
+    Blocks with an infinity or a NaN become NaN as a whole.  The last block of a K that 32 does not divide is filled with zeros.  No
+    gradient flows through it."""
     if isinstance(x, Planes):
         dev = _dev(x.hi, "x")
         q = Mxfp4._new(x.M, x.K, x.hi.device, (x.M, x.K))
@@ -124,7 +125,8 @@ def linear_mxfp4(x: Union[torch.Tensor, Mxfp4, Planes], w: Mxfp4, bias: Optional
     encoder's operand planes) or comes as an Mxfp4,
     w = quantize_mxfp4(weight [N, K]) once per checkpoint, bias [N] float32, act one of ops.ACT_*.  The result [..., N] has x's type
     (float32 for an Mxfp4 or planes) unless out_dtype says otherwise; quantized=True returns quantize_mxfp4 of the float32 result instead (an operand
-    of the next layer; written by the product itself where N is a multiple of 256).  No gradient flows through it."""
+    of the next layer; written by the product itself where N is a multiple of 256).  Inference only: an x that requires a gradient is
+    refused under grad mode, weight and bias get none."""
     if isinstance(x, Planes):
         x = quantize_mxfp4(x)
     if not isinstance(w, Mxfp4) or len(w.shape) != 2:
@@ -132,6 +134,8 @@ def linear_mxfp4(x: Union[torch.Tensor, Mxfp4, Planes], w: Mxfp4, bias: Optional
     if not isinstance(x, Mxfp4):
         if not isinstance(x, torch.Tensor) or x.dtype not in DTYPE_CODE:
             raise TypeError(f"linear_mxfp4: x is float32, bfloat16, float16 or an Mxfp4, got {getattr(x, 'dtype', type(x))}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("linear_mxfp4: x requires a gradient, and none flows through the product (torch.no_grad(), or x.detach())")
     if len(x.shape) < 1 or x.shape[-1] != w.K:
         raise ValueError(f"linear_mxfp4: x {tuple(x.shape)} does not end in the weight's {w.K} columns")
     if w.M < 1:

@@ -91,3 +91,17 @@ def test_the_library_refuses_before_any_launch():
     # calls without work need no memory
     assert lib.snf_mxfp4_quantize(None, 0, 0, 64, 64, None, None, None) == 0
     assert lib.snf_mxfp4_linear(None, None, None, None, None, 0, 64, 8, 0, None, 0, None) == 0
+
+
+def test_linear_refuses_to_drop_a_gradient():
+    """No gradient flows through the product: an x that asks for one is refused, unless nothing is recorded."""
+    from samnerf_amd import ops
+    w = ops.Mxfp4(*_codes(8, 64), 64)
+    x = torch.zeros((2, 64), requires_grad=True)
+    for kw in ({}, dict(quantized=True)):
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            ops.linear_mxfp4(x, w, **kw)
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            ops.linear_mxfp4(x.detach(), w, **kw)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+            ops.linear_mxfp4(x, w, **kw)
