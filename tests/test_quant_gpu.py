@@ -512,3 +512,61 @@ def test_encoder_weights_that_are_replaced():
         assert torch.equal(enc._wmxfp4(lin).float(), ops.quantize_mxfp4(lin.weight.detach()).float())
         hi, lo = enc._wplanes(lin)
         assert bool((hi.float() + lo.float() == i + 1).all())
+
+
+@pytest.mark.parametrize("embed", [64, 256])  # the plain path and the one on operand planes
+def test_encoder_layers_are_fed_and_used_as_the_block_says(embed, monkeypatch):
+    """The blocks' formulas in 64 bits around the layers' own results: the encoder in 4 bits hands every dense layer the operand that the
+    formulas make of the results before it (norms, windows, attention, residuals: 2^-16 of a product's operands, scores up to 10, so 2e-3
+    of the largest value), lin1 alone applies the GELU, and its result is the quantised product of its operands; what comes out is what the
+    formulas make of the last results."""
+    from samnerf_amd import ops
+    from oracle import vit_oracle as V
+    enc = _small_encoder(embed).set_linear_format("mxfp4")
+    x = torch.randn((2, 3, 224, 224), generator=torch.Generator().manual_seed(3)).cuda()
+    real, calls = ops.linear_mxfp4, []
+
+    def recorded(a, w, bias=None, act=0, **kw):
+        r = real(a, w, bias, act, **kw)
+        rows = lambda t: t.float().cpu().double().clone()  # noqa: E731  (operand planes are written again by the next block)
+        calls.append((rows(a), rows(w), None if bias is None else rows(bias.detach()), act, isinstance(a, ops.Mxfp4), isinstance(r, ops.Mxfp4), rows(r)))
+        return r
+
+    monkeypatch.setattr(ops, "linear_mxfp4", recorded)
+    y, trace = enc(x, trace_blocks=(0, 1))
+    names = ["qkv", "proj", "lin1", "lin2"] * 2
+    assert len(calls) == 8 and [c[3] for c in calls] == [ops.ACT_GELU if n == "lin1" else ops.ACT_NONE for n in names]
+    # lin1: the codes of its float32 result (a sum next to a border may fall on the other side: test_linear_quantized_result)
+    for (a, w, b, act, _, codes, r), n in zip(calls, names):
+        assert codes == (n == "lin1")
+        if codes:
+            values = lambda t: torch.from_numpy(reference(t)[2])  # noqa: E731
+            want = values(act64(values(a) @ w.t() + b, 3).float())
+            assert bool(((r - want).abs() <= want.abs().amax(1, keepdim=True) / 2).all()) and float((r != want).double().mean()) <= 0.01
+            dropped = values((values(a) @ w.t() + b).float())
+            assert float((r != dropped).double().mean()) > 0.3  # (the comparison sees a missing GELU)
+    left = list(zip(calls, names))
+
+    class Formulas:
+        layer_norm, pad, conv2d = torch.nn.functional.layer_norm, torch.nn.functional.pad, torch.nn.functional.conv2d
+        gelu = staticmethod(lambda t: t)  # (lin1's results are after it)
+
+        @staticmethod
+        def linear(t, w, b):
+            (a, wv, bv, _, coded, _, r), n = left.pop(0)
+            got = a.reshape(-1, w.shape[1])
+            rows = t.reshape(-1, w.shape[1])
+            assert got.shape == rows.shape and float((got - rows).abs().max()) <= (0 if coded else 2e-3 * float(rows.abs().max())), n
+            assert coded == (n == "lin2")
+            assert torch.equal(wv, torch.from_numpy(reference(w)[2])) and torch.equal(bv, b)
+            return r.reshape(*t.shape[:-1], w.shape[0])
+
+    monkeypatch.setattr(V, "F", Formulas)
+    cfg = V.ViTConfig(img_size=224, patch_size=16, embed_dim=embed, depth=2, num_heads=4, mlp_ratio=2.0, out_chans=32, window_size=5,
+                      global_attn_indexes=(1,))
+    sd = {k: v.detach().cpu().double() for k, v in enc.state_dict().items()}
+    want, tokens = V.forward(sd, x.cpu().double(), cfg, return_tokens=True)
+    assert not left
+    for i in (0, 1):
+        assert float((trace[i].cpu().double() - tokens[i + 1]).abs().max()) <= 2e-3 * float(tokens[i + 1].abs().max())
+    assert float((y.cpu().double() - want).abs().max()) <= 2e-3 * float(want.abs().max())
