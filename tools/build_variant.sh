@@ -6,6 +6,7 @@ cd "$(dirname "$0")/.."
 NAME=$1; FILES=$2; FLAGS=$3
 PKG=segment-anything-in-nerf_amd
 python -c "import sys; sys.path.insert(0,'.'); import samnerf_amd; from samnerf_amd import _lib; _lib.build()"
+HIPCC_FLAGS=$(python -c "import sys; sys.path.insert(0,'.'); import samnerf_amd; from samnerf_amd import _lib; print(' '.join(_lib.HIPCC_FLAGS))")
 mkdir -p tools/ab /tmp/snf_variant_$NAME
 OBJS=""
 for o in $PKG/lib/obj/*.o; do
@@ -14,7 +15,7 @@ for o in $PKG/lib/obj/*.o; do
   [ $skip = 0 ] && OBJS="$OBJS $o"
 done
 for f in $FILES; do
-  hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics $FLAGS -w -I include -c $PKG/csrc/$f -o /tmp/snf_variant_$NAME/${f%.hip}.o &
+  hipcc $HIPCC_FLAGS $FLAGS -w -I include -c $PKG/csrc/$f -o /tmp/snf_variant_$NAME/${f%.hip}.o &
 done
 wait
 for f in $FILES; do OBJS="$OBJS /tmp/snf_variant_$NAME/${f%.hip}.o"; done

@@ -3,7 +3,8 @@
 # usage: tools/kernel_resources.sh [file.hip ...]   (default: all of csrc/)
 cd "$(dirname "$0")/../segment-anything-in-nerf_amd/csrc"
 files=${@:-*.hip}
-for f in $files; do /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -I ../../include $EXTRA -c $f -o /tmp/kr_$$.o -Rpass-analysis=kernel-resource-usage 2>&1 | python3 -c "
+HIPCC_FLAGS=$(cd ../.. && python3 -c "import samnerf_amd; from samnerf_amd import _lib; print(' '.join(_lib.HIPCC_FLAGS))")
+for f in $files; do /opt/rocm/bin/hipcc $HIPCC_FLAGS -I ../../include $EXTRA -c $f -o /tmp/kr_$$.o -Rpass-analysis=kernel-resource-usage 2>&1 | python3 -c "
 import sys,re,subprocess
 cur=None; rows={}
 for l in sys.stdin:
