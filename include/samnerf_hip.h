@@ -556,7 +556,8 @@ int snf_top_distill_bwd(const void* z, int dtype, int R, int V, int64_t ld, cons
  * snf_mxfp4_linear_quantized: the result as the next product's operand, codes and scales of act(a w^T + bias) as snf_mxfp4_quantize would
  *   make them from its fp32 values; N a multiple of 256.
  * snf_mxfp4_linear_rows: snf_mxfp4_linear for up to SNF_MXFP4_ROWS rows x [M, K] of `dtype` (rows `ld` elements apart) that are quantised on the
- *   way into the product: one launch.  The same result as snf_mxfp4_quantize followed by snf_mxfp4_linear. */
+ *   way into the product: one launch.  The result of snf_mxfp4_quantize followed by snf_mxfp4_linear, up to the order of the fp32 sums (from
+ *   N = 8065 on the latter takes another kernel). */
 #define SNF_MXFP4_ROWS 16
 int snf_mxfp4_quantize(const void* x, int dtype, int M, int K, int64_t ld, uint8_t* codes, uint8_t* scales, snf_stream_t stream);
 int snf_mxfp4_quantize_planes(const uint16_t* hi, const uint16_t* lo, int M, int K, uint8_t* codes, uint8_t* scales, snf_stream_t stream);

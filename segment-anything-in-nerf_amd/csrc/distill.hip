@@ -3,8 +3,8 @@
 //   snf_top_distill_*  : T^2 KL(teacher || student) per row, from the teacher's top logits (and the mass of the rest, as one class of its
 //                        own), with the student's gradient
 // Bound by reading the rows: a part of a row stays in registers (16 bytes a load, all under way at once) while its maximum and its sum of
-// exponentials are taken; rows may begin at any element of a 16-byte granule.  4096 rows of 65536 bf16, k = 64: selection 138 us (streaming
-// 91 us = 5.9 TB/s, then 47), loss 150 us (4.1 TB/s), gradient 180 us (1.07 GB, 5.9 TB/s).
+// exponentials are taken; rows may begin at any element of a 16-byte granule.  4096 rows of 65536 bf16, k = 64 (medians): selection 142 us
+// (streaming 94 us = 5.7 TB/s, then 48), loss 166 us (reading 144 us = 3.7 TB/s, then 17 + 5), gradient 179 us (1.07 GB, 6.0 TB/s).
 #include "common.hpp"
 
 namespace snf {
@@ -988,8 +988,8 @@ constexpr int td_capacity(int shape, int E) { return TD_SHAPES[shape].threads * 
 struct TdPlan { int shape, parts, part_len; };
 
 // Loss: the smallest wave that holds a row; long rows are dealt out in parts of 8 KB, a wave each (no barriers, and every wave's loads are
-// under way at once: 4096 x 65536 bf16 in 150 us with workgroups of 256 threads x 16 KB, 130 with waves), of 4 KB where that makes fewer
-// than 256 of them.
+// under way at once: 4096 x 65536 bf16, in turn and at their best, in 150 us with workgroups of 256 threads x 16 KB, 130 with waves), of
+// 4 KB where that makes fewer than 256 of them.
 static TdPlan td_rows_plan(int R, int V, int E) {
     int s = 0;
     while (s < 2 && td_capacity(s, E) < V) ++s;
@@ -1032,7 +1032,8 @@ static int td_top_t(const T* x, int R, int V, int64_t ld, int k, float temperatu
     }
 #undef TD_GO
     const int groups = td_top_group_count(V, E), granules = groups * TD_GROUP;
-    // 16 KB a workgroup; 4 KB where that makes fewer than 1024 of them
+    // 16 KB a workgroup; 4 KB where that makes fewer than 1024 of them (64 x 65536 bf16, k = 64: both kernels 17.6 us with 4 KB, 18.3 with
+    // 16; from 120 such rows on, and for one row of 32000 or 10^6 fp32, within the 3 % that two runs differ by)
     const int64_t big = (int64_t)R * ceil_div(granules, 256 * 4);
     const int per = big < 1024 ? 64 * 4 : 256 * 4, chunks = ceil_div(granules, per);
     SNF_REQUIRE((int64_t)R * chunks * (per / 4) < ((int64_t)1 << 32), "snf_top_logits: %d rows of %d are too many for one launch", R, V);

@@ -257,8 +257,8 @@ constexpr int mx_stage(int bm, int bn) { return (8 * 16 + 2 * 4) * (bm + bn); }
 // ends up with four consecutive columns of one row, and the tile leaves through LDS in whole rows of 64 columns, where the bias and the
 // activation are applied; its stores do not stay in the caches (they are half of a wide layer's time: 4900 x 1280 -> 3840 fp32 36 us with
 // ordinary stores, 32 with these).
-// Measured: 4900 x 1280 -> 3840 fp32 (75 MB out) 30 us = 1.6 PFLOP/s, 2.5 TB/s of stores: stores, copies and products a third each;
-// 16384 x 5120 -> 5120 bf16 225 us = 3.8 PFLOP/s: a tile's 256 k take 1.9 us, its products alone 1.3, its copies through L2 alone 1.0.
+// Measured (medians): 4900 x 1280 -> 3840 fp32 (75 MB out) 32 us = 1.5 PFLOP/s, 2.3 TB/s of stores: stores, copies and products a third each;
+// 16384 x 5120 -> 5120 bf16 227 us = 3.8 PFLOP/s: a tile's 256 k take 1.9 us, its products alone 1.3, its copies through L2 alone 1.0.
 template <int BM, int BN, int WM, int WN, typename T>
 __global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_linear(const uint8_t* __restrict__ a, const uint8_t* __restrict__ as,
                                                                const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
